@@ -270,6 +270,39 @@ int llmopt_cuda_w4a16_linear(llmopt_cuda_context* context, const void* input, co
                              const void* scale, const void* bias, void* output, int64_t m, int64_t n, int64_t k,
                              void* stream);
 
+/* ---- MXFP4 on raw device pointers ------------------------------------------------------ */
+
+/* No counterparts in the reference.  Microscaled 4-bit floating point (OCP Microscaling: e2m1 elements, one e8m0 power of
+ * two per 32 of them along k): rows [rows, k] are held as
+ *   codes  u8 [rows, k / 2], the element of even k in the low nibble, 16-byte aligned, and
+ *   scales u32 [ceil(k / 128), rows]: byte j of word (g, r) is the exponent (plus 127; 255: no number) of block 4 g + j of row r;
+ * k is a multiple of 32.  The kernels of the same names (llmopt_mxfp4_quantize_f16 and so on) do the same for buffers in
+ * batches and plans; these run one of them on `stream` (a cudaStream_t; NULL = the context's) of the context's device without waiting,
+ * keep nothing between calls and use no memory but the operands, so calls on different streams may overlap and a stream capture
+ * may hold them.  `type`: what the operand without codes is held in. */
+#define LLMOPT_CUDA_F16 0
+#define LLMOPT_CUDA_BF16 1
+#define LLMOPT_CUDA_F32 2
+
+/* x [rows, k], row i at x + i * stride elements, to codes and scales.  With row_of_slot (u32 [rows]; an index beyond the rows counts as
+ * the last one) row i is x's row row_of_slot[i] of source_rows.  An exponent is that of the block's largest size minus 2 (which
+ * saturates beyond 6 units), elements round to nearest, ties to even; a block with an infinity or NaN becomes one of NaNs. */
+int llmopt_cuda_mxfp4_quantize(llmopt_cuda_context* context, int type, const void* x, const void* row_of_slot, void* codes,
+                               void* scales, int64_t rows, int64_t source_rows, int64_t k, int64_t stride, void* stream);
+/* The values [rows, k], rounded once to `type`. */
+int llmopt_cuda_mxfp4_dequantize(llmopt_cuda_context* context, int type, const void* codes, const void* scales, void* out,
+                                 int64_t rows, int64_t k, void* stream);
+/* out [m, n] = x [m, k] . w [n, k]^T + bias [n] (may be NULL), sums in fp32; bias and out in `type`. */
+int llmopt_cuda_mxfp4_linear(llmopt_cuda_context* context, int type, const void* x_codes, const void* x_scales,
+                             const void* w_codes, const void* w_scales, const void* bias, void* out, int64_t m, int64_t n,
+                             int64_t k, void* stream);
+/* Rows sorted by expert (slots of them, as llmopt_route_plan sorts and lists them) times their experts' n rows of w
+ * [experts * n, k].  paired: neighbouring columns are a gate and a value, out [slots, n / 2] in `type` (f16 or bf16) =
+ * silu(score * gate) * (score * value); otherwise out is f32 [slots, n] and score_of_slot is not read. */
+int llmopt_cuda_mxfp4_expert_rows(llmopt_cuda_context* context, int type, const void* x_codes, const void* x_scales,
+                                  const void* w_codes, const void* w_scales, const void* plan, const void* score_of_slot,
+                                  void* out, int64_t slots, int64_t n, int64_t k, int64_t experts, int paired, void* stream);
+
 /* ---- entry point that allocates nothing ---------------------------------------------- */
 
 /* No counterpart in the reference. For hosts that cannot let the library allocate

@@ -85,6 +85,7 @@ LLMOPT_FAMILY const NamedLauncher* sequence_glue_launchers(size_t* count);
 LLMOPT_FAMILY const NamedLauncher* row_attention_launchers(size_t* count);
 LLMOPT_FAMILY const NamedLauncher* matrix_state_launchers(size_t* count);
 LLMOPT_FAMILY const NamedLauncher* expert_launchers(size_t* count);
+LLMOPT_FAMILY const NamedLauncher* mxfp4_launchers(size_t* count);
 struct ExprProgram {
   uint8_t code[192];
   uint32_t length;
@@ -387,7 +388,7 @@ static void register_kernels(llmopt_cuda_library* library) {
   // the sequence-mixer kernels
   const NamedLauncher* (*const families[])(size_t*) = {norm_family_launchers, dense_linear_launchers,
                                                        sequence_glue_launchers, row_attention_launchers,
-                                                       matrix_state_launchers, expert_launchers};
+                                                       matrix_state_launchers, expert_launchers, mxfp4_launchers};
   for (auto family : families) {
     size_t count = 0;
     const NamedLauncher* table = family != nullptr ? family(&count) : nullptr;
@@ -1611,6 +1612,122 @@ int llmopt_cuda_w4a16_linear(llmopt_cuda_context* context, const void* input, co
     return set_error(LLMOPT_CUDA_FAILURE, "this library was linked without the W4A16 kernels");
   if (launch_w4a16_linear(args) != 0) return set_error(LLMOPT_CUDA_FAILURE, message);
   return LLMOPT_CUDA_OK;
+}
+
+// ---- MXFP4 on raw device pointers ------------------------------------------------------
+
+namespace {
+// The operands of a launch whose pointers are the caller's: their extents follow from the sizes, and the launcher of the name
+// makes the checks that a dispatch of it gets.
+struct PointerLaunch {
+  KernelArgs args = {};
+  std::string message;
+  uint32_t params[5] = {};
+  bool null_pointer = false, too_large = false;
+
+  PointerLaunch(Context* context, void* stream) {
+    args.ctx = context;
+    args.stream = stream ? (cudaStream_t)stream : context->stream;
+    args.params = (const uint8_t*)params;
+    args.error = &message;
+  }
+  void operand(const void* pointer, size_t bytes) {
+    null_pointer |= pointer == nullptr && bytes > 0;
+    args.buffers[args.buffer_count] = (void*)pointer;
+    args.lengths[args.buffer_count++] = bytes;
+  }
+  void sizes(std::initializer_list<int64_t> values) {
+    for (int64_t value : values) {
+      too_large |= value < 0 || value > 0x7fffffff;
+      params[args.param_bytes / 4] = (uint32_t)value;
+      args.param_bytes += 4;
+    }
+  }
+  int run(const std::string& name) {
+    if (too_large) return set_error(LLMOPT_CUDA_INVALID_ARGUMENT, name + ": a size is negative or too large");
+    if (null_pointer) return set_error(LLMOPT_CUDA_INVALID_ARGUMENT, name + " received a null tensor");
+    size_t count = 0;
+    const NamedLauncher* table = mxfp4_launchers != nullptr ? mxfp4_launchers(&count) : nullptr;
+    if (table == nullptr) return set_error(LLMOPT_CUDA_FAILURE, "this library was linked without the MXFP4 kernels");
+    const NamedLauncher* found = table;
+    while (found != table + count && name != found->name) ++found;
+    if (found == table + count) return set_error(LLMOPT_CUDA_INVALID_ARGUMENT, name + " is no kernel");
+    args.name = found->name;
+    int current = -1;
+    CUDA_TRY(cudaGetDevice(&current), "cudaGetDevice failed");
+    if (current != args.ctx->device) CUDA_TRY(cudaSetDevice(args.ctx->device), "cudaSetDevice failed");
+    const int status = found->launcher(args);
+    if (current != args.ctx->device) cudaSetDevice(current);
+    if (status != 0) return set_error(LLMOPT_CUDA_INVALID_ARGUMENT, message);
+    return LLMOPT_CUDA_OK;
+  }
+};
+const char* mxfp4_suffix(int type) {
+  return type == LLMOPT_CUDA_F16 ? "_f16" : type == LLMOPT_CUDA_BF16 ? "_bf16" : type == LLMOPT_CUDA_F32 ? "_f32" : "_?";
+}
+size_t mxfp4_size(int type) { return type == LLMOPT_CUDA_F32 ? 4 : 2; }
+// Extents of rows in 4 bits; sizes that are refused later count as nothing.
+size_t mxfp4_extent(int64_t rows, int64_t per_row) {
+  return rows > 0 && per_row > 0 && rows <= 0x7fffffff && per_row <= 0x7fffffff ? (size_t)rows * (size_t)per_row : 0;
+}
+size_t mxfp4_codes(int64_t rows, int64_t k) { return mxfp4_extent(rows, k / 2); }
+size_t mxfp4_scales(int64_t rows, int64_t k) { return mxfp4_extent(rows, (k + 127) / 128) * 4; }
+}  // namespace
+
+int llmopt_cuda_mxfp4_quantize(llmopt_cuda_context* context, int type, const void* x, const void* row_of_slot, void* codes, void* scales,
+                               int64_t rows, int64_t source_rows, int64_t k, int64_t stride, void* stream) {
+  if (context == nullptr) return set_error(LLMOPT_CUDA_FAILURE, "CUDA context has been finalized");
+  PointerLaunch launch(context, stream);
+  const int64_t read = row_of_slot ? source_rows : rows;
+  launch.operand(x, (read > 0 ? mxfp4_extent(read - 1, stride) + mxfp4_extent(1, k) : 0) * mxfp4_size(type));
+  if (row_of_slot) launch.operand(row_of_slot, mxfp4_extent(rows, 4));
+  launch.operand(codes, mxfp4_codes(rows, k));
+  launch.operand(scales, mxfp4_scales(rows, k));
+  launch.sizes({rows, k, stride});
+  if (row_of_slot) launch.sizes({source_rows});
+  return launch.run(std::string(row_of_slot ? "llmopt_mxfp4_quantize_rows" : "llmopt_mxfp4_quantize") + mxfp4_suffix(type));
+}
+
+int llmopt_cuda_mxfp4_dequantize(llmopt_cuda_context* context, int type, const void* codes, const void* scales, void* out, int64_t rows,
+                                 int64_t k, void* stream) {
+  if (context == nullptr) return set_error(LLMOPT_CUDA_FAILURE, "CUDA context has been finalized");
+  PointerLaunch launch(context, stream);
+  launch.operand(codes, mxfp4_codes(rows, k));
+  launch.operand(scales, mxfp4_scales(rows, k));
+  launch.operand(out, mxfp4_extent(rows, k) * mxfp4_size(type));
+  launch.sizes({rows, k});
+  return launch.run(std::string("llmopt_mxfp4_dequantize") + mxfp4_suffix(type));
+}
+
+int llmopt_cuda_mxfp4_linear(llmopt_cuda_context* context, int type, const void* x_codes, const void* x_scales, const void* w_codes,
+                             const void* w_scales, const void* bias, void* out, int64_t m, int64_t n, int64_t k, void* stream) {
+  if (context == nullptr) return set_error(LLMOPT_CUDA_FAILURE, "CUDA context has been finalized");
+  PointerLaunch launch(context, stream);
+  launch.operand(x_codes, mxfp4_codes(m, k));
+  launch.operand(x_scales, mxfp4_scales(m, k));
+  launch.operand(w_codes, mxfp4_codes(n, k));
+  launch.operand(w_scales, mxfp4_scales(n, k));
+  launch.operand(bias, bias ? mxfp4_extent(n, 1) * mxfp4_size(type) : 0);
+  launch.operand(out, mxfp4_extent(m, n) * mxfp4_size(type));
+  launch.sizes({m, n, k, bias != nullptr});
+  return launch.run(std::string("llmopt_mxfp4_linear") + mxfp4_suffix(type));
+}
+
+int llmopt_cuda_mxfp4_expert_rows(llmopt_cuda_context* context, int type, const void* x_codes, const void* x_scales, const void* w_codes,
+                                  const void* w_scales, const void* plan, const void* score_of_slot, void* out, int64_t slots, int64_t n,
+                                  int64_t k, int64_t experts, int paired, void* stream) {
+  if (context == nullptr) return set_error(LLMOPT_CUDA_FAILURE, "CUDA context has been finalized");
+  PointerLaunch launch(context, stream);
+  const int64_t w_rows = (int64_t)std::min<size_t>(mxfp4_extent(experts, n), (size_t)1 << 31);
+  launch.operand(x_codes, mxfp4_codes(slots, k));
+  launch.operand(x_scales, mxfp4_scales(slots, k));
+  launch.operand(w_codes, mxfp4_codes(w_rows, k));
+  launch.operand(w_scales, mxfp4_scales(w_rows, k));
+  launch.operand(plan, slots > 0 ? 16 * (1 + (size_t)(slots / 128) + (size_t)std::min(slots, experts)) : 0);
+  launch.operand(score_of_slot, paired ? mxfp4_extent(slots, 4) : 0);
+  launch.operand(out, paired ? mxfp4_extent(slots, n / 2) * mxfp4_size(type) : mxfp4_extent(slots, n) * 4);
+  launch.sizes({slots, n, k, experts, paired != 0});
+  return launch.run(std::string("llmopt_mxfp4_expert_rows") + mxfp4_suffix(type));
 }
 
 namespace llmopt {

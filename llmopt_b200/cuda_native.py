@@ -117,6 +117,10 @@ SIGNATURES = {
     "llmopt_cuda_measure_hardware": (_I, [_I, _I, _I, _I64, ctypes.c_char_p, _SZ, ctypes.POINTER(_I),
                                          ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]),
     "llmopt_cuda_w4a16_linear": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P]),
+    "llmopt_cuda_mxfp4_quantize": (_I, [_P, _I, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P]),
+    "llmopt_cuda_mxfp4_dequantize": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _P]),
+    "llmopt_cuda_mxfp4_linear": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P]),
+    "llmopt_cuda_mxfp4_expert_rows": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P]),
     "llmopt_cuda_attention_q8_paged_static": (_I, [_P, _P, _P, _P, _P, _P, _P, _SZ, ctypes.c_uint32, _P]),
     "llmopt_cuda_time_dispatch": (_I, [_P, _REC, _I, _I, _I, ctypes.POINTER(ctypes.c_float)]),
     "llmopt_cuda_time_dispatches": (_I, [_P, _REC, _SZ, _I, _I, ctypes.POINTER(ctypes.c_float)]),
@@ -407,6 +411,34 @@ class Runtime:
         """The Python single-op boundary (native/metal_runtime.cpp:58-136) on raw device pointers."""
         _check(load_library().llmopt_cuda_w4a16_linear(
             self._context, x_ptr, packed_ptr, scale_ptr, bias_ptr or None, out_ptr, m, n, k, stream or None))
+
+    # MXFP4 operators on raw device pointers and a caller's stream (0: the context's), without waiting; formats and rounding:
+    # include/llmopt_cuda.h. ``element`` is "f16", "bf16" or "f32": what the operand outside of the 4-bit format is held in.
+    _ELEMENTS = {"f16": 0, "bf16": 1, "f32": 2}
+
+    def mxfp4_quantize_pointers(self, element: str, x_ptr: int, row_of_slot_ptr: Optional[int], codes_ptr: int, scales_ptr: int,
+                                rows: int, source_rows: int, k: int, stride: int, stream: int = 0) -> None:
+        _check(load_library().llmopt_cuda_mxfp4_quantize(
+            self._context, self._ELEMENTS[element], x_ptr, row_of_slot_ptr or None, codes_ptr, scales_ptr, rows, source_rows, k, stride,
+            stream or None))
+
+    def mxfp4_dequantize_pointers(self, element: str, codes_ptr: int, scales_ptr: int, out_ptr: int, rows: int, k: int,
+                                  stream: int = 0) -> None:
+        _check(load_library().llmopt_cuda_mxfp4_dequantize(
+            self._context, self._ELEMENTS[element], codes_ptr, scales_ptr, out_ptr, rows, k, stream or None))
+
+    def mxfp4_linear_pointers(self, element: str, x_codes_ptr: int, x_scales_ptr: int, w_codes_ptr: int, w_scales_ptr: int,
+                              bias_ptr: Optional[int], out_ptr: int, m: int, n: int, k: int, stream: int = 0) -> None:
+        _check(load_library().llmopt_cuda_mxfp4_linear(
+            self._context, self._ELEMENTS[element], x_codes_ptr, x_scales_ptr, w_codes_ptr, w_scales_ptr, bias_ptr or None, out_ptr,
+            m, n, k, stream or None))
+
+    def mxfp4_expert_rows_pointers(self, element: str, x_codes_ptr: int, x_scales_ptr: int, w_codes_ptr: int, w_scales_ptr: int,
+                                   plan_ptr: int, score_of_slot_ptr: Optional[int], out_ptr: int, slots: int, n: int, k: int,
+                                   experts: int, paired: bool, stream: int = 0) -> None:
+        _check(load_library().llmopt_cuda_mxfp4_expert_rows(
+            self._context, self._ELEMENTS[element], x_codes_ptr, x_scales_ptr, w_codes_ptr, w_scales_ptr, plan_ptr,
+            score_of_slot_ptr or None, out_ptr, slots, n, k, experts, int(paired), stream or None))
 
     def __del__(self):
         lib = _lib

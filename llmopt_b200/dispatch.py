@@ -336,6 +336,96 @@ def dispatch_quant_gated_linear(context: Context, *, m: int, n: int, k: int, inp
                  parameters.u32s([m, n, k, codes[activation]]), (linear_f16_grid(m * n), 1, 1))]
 
 
+# ---- MXFP4 (csrc/mxfp4.cuh has the format; no counterparts in the reference) --------------
+
+_MXFP4_ELEMENTS = {"float16": "f16", "bfloat16": "bf16", "float32": "f32"}
+
+
+def mxfp4_scale_words(k: int) -> int:
+    """Words of exponents that a row of ``k`` elements has."""
+    return (k + 127) // 128
+
+
+def _mxfp4_operand_ok(codes: Tensor, scales: Tensor, rows: int, k: int) -> bool:
+    return (codes.dtype == "uint8" and tuple(codes.shape) == (rows, k // 2) and scales.dtype == "uint32"
+            and tuple(scales.shape) == (mxfp4_scale_words(k), rows))
+
+
+def _mxfp4_element(tensor: Tensor, most: str) -> str:
+    element = _MXFP4_ELEMENTS.get(tensor.dtype)
+    if element is None or (most == "16" and element == "f32"):
+        raise DispatchError(f"MXFP4 kernels take no {tensor.dtype} here")
+    return element
+
+
+def dispatch_mxfp4_quantize(context: Context, *, input: Tensor, codes: Tensor, scales: Tensor, row_of_slot: Optional[Tensor] = None,
+                            columns: Optional[int] = None) -> list:
+    """Rows of ``input`` [rows, stride] (their first ``columns``, all if None) to ``codes`` u8 [slots, k / 2] and ``scales`` u32
+    [ceil(k / 128), slots]; with ``row_of_slot`` u32 [slots] the rows that it names, as routed experts read them."""
+    element = _mxfp4_element(input, "32")
+    if len(input.shape) != 2:
+        raise DispatchError("MXFP4 quantization input must have rank two")
+    source_rows, stride = input.shape
+    k = stride if columns is None else columns
+    slots = source_rows if row_of_slot is None else row_of_slot.numel
+    if not 0 < k <= stride or k % 32 != 0:
+        raise DispatchError(f"MXFP4 quantization needs whole blocks of 32, got {k} columns of {stride}")
+    if not _mxfp4_operand_ok(codes, scales, slots, k) or (row_of_slot is not None and row_of_slot.dtype != "uint32"):
+        raise DispatchError("MXFP4 quantization metadata is inconsistent")
+    if row_of_slot is None:
+        return [_run(context, f"llmopt_mxfp4_quantize_{element}", [input.buffer, codes.buffer, scales.buffer],
+                     parameters.mxfp4_quantize(rows=slots, k=k, stride=stride), (1, 1, 1))]
+    return [_run(context, f"llmopt_mxfp4_quantize_rows_{element}", [input.buffer, row_of_slot.buffer, codes.buffer, scales.buffer],
+                 parameters.mxfp4_quantize_rows(rows=slots, k=k, stride=stride, source_rows=source_rows), (1, 1, 1))]
+
+
+def dispatch_mxfp4_dequantize(context: Context, *, codes: Tensor, scales: Tensor, output: Tensor) -> list:
+    """The values of ``codes`` and ``scales``, rounded once to the type of ``output`` [rows, k]."""
+    element = _mxfp4_element(output, "32")
+    if len(output.shape) != 2 or output.shape[1] % 32 != 0 or not _mxfp4_operand_ok(codes, scales, *output.shape):
+        raise DispatchError("MXFP4 dequantization metadata is inconsistent")
+    rows, k = output.shape
+    return [_run(context, f"llmopt_mxfp4_dequantize_{element}", [codes.buffer, scales.buffer, output.buffer],
+                 parameters.mxfp4_dequantize(rows=rows, k=k), (1, 1, 1))]
+
+
+def dispatch_mxfp4_linear(context: Context, *, input: Tensor, input_scales: Tensor, weight: Tensor, weight_scales: Tensor,
+                          output: Tensor, bias: Optional[Tensor] = None) -> list:
+    """``output`` [m, n] = ``input`` [m, k] . ``weight`` [n, k]^T (+ ``bias`` [n], in the output's type), both in MXFP4, sums in fp32."""
+    element = _mxfp4_element(output, "32")
+    m, n, k = input.shape[0], weight.shape[0], 2 * weight.shape[1]
+    if k % 32 != 0 or not (_mxfp4_operand_ok(input, input_scales, m, k) and _mxfp4_operand_ok(weight, weight_scales, n, k)):
+        raise DispatchError("MXFP4 linear operands are inconsistent")
+    if tuple(output.shape) != (m, n) or (bias is not None and (bias.dtype != output.dtype or bias.numel != n)):
+        raise DispatchError("MXFP4 linear output or bias is inconsistent")
+    buffers = [input.buffer, input_scales.buffer, weight.buffer, weight_scales.buffer, (output if bias is None else bias).buffer,
+               output.buffer]
+    return [_run(context, f"llmopt_mxfp4_linear_{element}", buffers,
+                 parameters.mxfp4_linear(m=m, n=n, k=k, has_bias=bias is not None), (linear_f16_grid(m * n), 1, 1))]
+
+
+def dispatch_mxfp4_expert_rows(context: Context, *, input: Tensor, input_scales: Tensor, weight: Tensor, weight_scales: Tensor,
+                               experts: int, plan: Buffer, output: Tensor, score_of_slot: Optional[Tensor] = None) -> list:
+    """Rows sorted by expert (``plan`` of ``llmopt_route_plan``) times their experts' matrices, ``weight`` [experts * n, k / 2].  With
+    ``score_of_slot`` f32 [slots] neighbouring columns are a gate and a value and ``output`` [slots, n / 2], f16 or bf16, is
+    silu(score * gate) * (score * value); without, it is f32 [slots, n]."""
+    paired = score_of_slot is not None
+    slots, k = input.shape[0], 2 * weight.shape[1]
+    if experts <= 0 or weight.shape[0] % experts != 0 or (paired and weight.shape[0] // experts % 2 != 0):
+        raise DispatchError("MXFP4 expert weights are no whole number of matrices")
+    n = weight.shape[0] // experts
+    if k % 32 != 0 or not (_mxfp4_operand_ok(input, input_scales, slots, k) and _mxfp4_operand_ok(weight, weight_scales, experts * n, k)):
+        raise DispatchError("MXFP4 expert operands are inconsistent")
+    if tuple(output.shape) != (slots, n // 2 if paired else n) or (not paired and output.dtype != "float32") or (
+            paired and (score_of_slot.dtype != "float32" or score_of_slot.numel != slots)):
+        raise DispatchError("MXFP4 expert output or scores are inconsistent")
+    element = _mxfp4_element(output, "16") if paired else "bf16"  # of fp32 rows there is one form
+    scores = score_of_slot.buffer if paired else plan
+    return [_run(context, f"llmopt_mxfp4_expert_rows_{element}", [input.buffer, input_scales.buffer, weight.buffer, weight_scales.buffer,
+                                                                  plan, scores, output.buffer],
+                 parameters.expert_rows(pairs=slots, n=n, k=k, experts=experts, paired=paired), (1, 1, 1))]
+
+
 def dispatch_attention(context: Context, *, causal: bool, scale: float, query: Tensor, key: Tensor, value: Tensor,
                        output: Tensor, mask: Optional[Tensor] = None) -> list:
     """dispatch_attention, lib/metal_dispatch_attention.ml:6-102: dense fp16 attention (prefill).

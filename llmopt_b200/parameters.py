@@ -207,6 +207,22 @@ def expert_rows(*, pairs, n, k, experts, paired) -> bytes:
     return u32s([pairs, n, k, experts, 1 if paired else 0])
 
 
+def mxfp4_quantize(*, rows, k, stride) -> bytes:
+    return u32s([rows, k, stride])
+
+
+def mxfp4_quantize_rows(*, rows, k, stride, source_rows) -> bytes:
+    return u32s([rows, k, stride, source_rows])
+
+
+def mxfp4_dequantize(*, rows, k) -> bytes:
+    return u32s([rows, k])
+
+
+def mxfp4_linear(*, m, n, k, has_bias) -> bytes:
+    return u32s([m, n, k, 1 if has_bias else 0])
+
+
 def expert_combine(*, rows, width, top) -> bytes:
     return u32s([rows, width, top])
 

@@ -90,3 +90,32 @@ def q4_0_blocks(scales, nibbles):
     out[:, :, 0:2] = scales.view(np.uint8).reshape(n, blocks, 2)
     out[:, :, 2:18] = grouped[:, :, :16] | (grouped[:, :, 16:] << 4)
     return out.reshape(n, blocks * 18)
+
+
+def mxfp4_scale_words(exponents: np.ndarray) -> np.ndarray:
+    """E8M0 exponents uint8 [rows, k / 32], as checkpoints hold them, to the words of the MXFP4 kernels: uint32
+    [ceil(k / 128), rows], block 4g + j of a row in byte j of word g."""
+    if exponents.ndim != 2 or exponents.dtype != np.uint8:
+        raise TypeError(f"MXFP4 exponents must be uint8 rows, got {exponents.dtype} {exponents.shape}")
+    rows, blocks = exponents.shape
+    padded = np.zeros((rows, (blocks + 3) // 4 * 4), np.uint8)
+    padded[:, :blocks] = exponents
+    return np.ascontiguousarray(padded.view("<u4").T)
+
+
+def pack_mxfp4_weight(weight: np.ndarray):
+    """fp [N, K] -> (codes u8 [N, K/2], scale words u32 [ceil(K/128), N]) on the host, with the rounding of
+    llmopt_mxfp4_quantize_*: exponent floor(log2 amax) - 2, e2m1 to nearest, ties to even, saturated at 6 units."""
+    if weight.ndim != 2 or weight.shape[1] == 0 or weight.shape[1] % 32 != 0:
+        raise ValueError(f"MXFP4 weight must be rows of whole blocks of 32, got shape {tuple(weight.shape)}")
+    n, k = weight.shape
+    blocks = weight.astype(np.float32).reshape(n, k // 32, 32)
+    finite = np.isfinite(blocks).all(axis=-1)
+    blocks = np.where(finite[..., None], blocks, np.float32(0.0))
+    most = np.abs(blocks).max(axis=-1)
+    shift = np.where(most > 0, np.clip(np.frexp(most)[1] - 3, -127, 127), -127)
+    size = np.abs(np.ldexp(blocks, -shift[..., None]))
+    code = np.where(size < 2, np.rint(size * 2), np.where(size < 4, np.rint(size) + 2, np.minimum(np.rint(size / 2) + 4, 7)))
+    code = np.where(finite[..., None], code.astype(np.uint8) | (np.signbit(blocks).astype(np.uint8) << 3), 0).astype(np.uint8).reshape(n, k)
+    exponents = np.where(finite, shift + 127, 255).astype(np.uint8)
+    return np.ascontiguousarray(code[:, 0::2] | (code[:, 1::2] << 4)), mxfp4_scale_words(exponents)
