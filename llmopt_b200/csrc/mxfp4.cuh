@@ -48,7 +48,6 @@ struct Problem {
   const float* row_scale;  // paired: multiplies a row's sums
   void* out;
   uint32_t m, n, k, w_rows;  // w_rows: rows of w, all experts'
-  uint32_t paired;           // columns 2j, 2j + 1 leave as silu(2j) * (2j + 1)
   DensePlan plan;            // rows sorted by expert
 };
 
