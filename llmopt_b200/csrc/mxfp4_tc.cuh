@@ -1,0 +1,155 @@
+// What the MXFP4 products on tcgen05 share: operand and instruction forms, the way sums leave, tensor maps.
+//
+// y[m, n] = sum over blocks b of 2^(sx + sw - 254) (x block . w block): the tensor cores take both operands as they are held, 64 elements
+// of k at a time with two powers of two per row (tcgen05.mma kind::mxf4), so no weight is ever converted.  The weights are the M side
+// (128 rows of a tile are the lanes of tensor memory, one output column each), the rows of x the N side: one token costs an N of 16,
+// and a ragged tile of an expert costs its rows rounded up to 16.
+#pragma once
+#include <cuda.h>
+
+#include "mxfp4.cuh"
+#include "w4a16_tc_device.cuh"
+
+namespace llmopt {
+
+uint32_t* context_device_error(Context* ctx);
+
+namespace mxfp4 {
+using namespace tc;
+
+constexpr uint32_t kColumns = 128, kDepth = 256, kRowBytes = kDepth / 2;  // weight rows of a tile, elements of k of a stage
+constexpr uint32_t kStageWords = kDepth / kWordValues, kAtom = 512;       // an atom: the words of 128 rows
+constexpr uint32_t kScaleWarps = 4;  // a thread per weight row
+
+// One lane of a converged warp.  What the tensor cores and copies take lies in uniform registers: where the whole warp walks through a loop
+// with values that are the same in all lanes and one lane issues, they are kept there; a loop that one lane walks through alone
+// moves every operand over, which cost 750 to 1000 cycles per four products.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t chosen;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(chosen));
+  return chosen != 0;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, barrier_wait(bar, parity)); }
+
+// kind::mxf4, e2m1 A and B (format 1), e8m0 scales, both K-major; `pair` picks the half of a scale word.
+__device__ __forceinline__ uint32_t mxf4_instruction(uint32_t n, uint32_t pair) {
+  return (pair << 5) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((kColumns >> 4) << 24) | (pair << 30);
+}
+__device__ __forceinline__ void mma_mxf4(uint32_t sums, uint64_t a, uint64_t b, uint32_t instruction, uint32_t a_scales, uint32_t b_scales,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+      ::"r"(sums), "l"(a), "l"(b), "r"(instruction), "r"(accumulate), "r"(a_scales), "r"(b_scales)
+      : "memory");
+}
+// An atom (32 rows of 16 bytes, unswizzled, eight rows every 128 bytes) to four columns, the same in all four quarters of the lanes.
+__device__ __forceinline__ void copy_atom(uint32_t columns, uint32_t shared_address) {
+  constexpr uint64_t kForm = (uint64_t)(128 >> 4) << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+  const uint64_t descriptor = kForm | (uint64_t)((shared_address & 0x3ffffu) >> 4);
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(columns), "l"(descriptor) : "memory");
+}
+
+enum Store : uint32_t { kStoreHalf, kStoreBf16, kStoreFloat, kStorePairHalf, kStorePairBf16 };
+template <Store S> struct Element { typedef float Type; };
+template <> struct Element<kStoreHalf> { typedef __half Type; };
+template <> struct Element<kStorePairHalf> { typedef __half Type; };
+template <> struct Element<kStoreBf16> { typedef bf16 Type; };
+template <> struct Element<kStorePairBf16> { typedef bf16 Type; };
+
+__device__ __forceinline__ uint32_t packed(__half a, __half b) { return (uint32_t)__half_as_ushort(a) | (uint32_t)__half_as_ushort(b) << 16; }
+__device__ __forceinline__ uint32_t packed(bf16 a, bf16 b) { return (uint32_t)__bfloat16_as_ushort(a) | (uint32_t)__bfloat16_as_ushort(b) << 16; }
+
+// Sums of COUNT rows from `row` on, of the output column that is this lane's, on their way out; the whole warp takes part.  Sixteen-bit
+// results go two columns at a time: neighbouring lanes exchange the sums of every other row.
+template <Store S, int COUNT>
+__device__ __forceinline__ void store_rows(const Problem& p, uint32_t row, uint32_t end, uint32_t column, const uint32_t (&raw)[COUNT]) {
+  typedef typename Element<S>::Type T;
+  const bool odd = threadIdx.x & 1u;
+  if constexpr (S == kStoreFloat) {
+    if (column >= p.n) return;
+    const float bias = p.bias ? reinterpret_cast<const float*>(p.bias)[column] : 0.0f;
+    float* out = reinterpret_cast<float*>(p.out) + (size_t)row * p.n + column;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i, out += p.n)
+      if (row + i < end) *out = __uint_as_float(raw[i]) + bias;
+  } else {
+    const uint32_t even_column = column & ~1u;
+    constexpr bool kPair = S == kStorePairHalf || S == kStorePairBf16;
+    float bias[2] = {};
+    if (!kPair && p.bias) {
+      if (even_column < p.n) bias[0] = as_float(reinterpret_cast<const T*>(p.bias)[even_column]);
+      if (even_column + 1u < p.n) bias[1] = as_float(reinterpret_cast<const T*>(p.bias)[even_column + 1u]);
+    }
+    const bool words = p.n % 2u == 0 && ((uintptr_t)p.out & 3u) == 0;
+#pragma unroll
+    for (int i = 0; i < COUNT; i += 2) {
+      const uint32_t away = __shfl_xor_sync(0xffffffffu, odd ? raw[i] : raw[i + 1], 1);
+      const float first = __uint_as_float(odd ? away : raw[i]), second = __uint_as_float(odd ? raw[i + 1] : away);
+      const uint32_t at = row + i + (odd ? 1 : 0);
+      if (at >= end || even_column >= p.n) continue;
+      if constexpr (kPair) {
+        const float scale = p.row_scale[at];
+        reinterpret_cast<T*>(p.out)[(size_t)at * (p.n / 2u) + even_column / 2u] = from_float<T>(silu_f32(first * scale) * (second * scale));
+      } else {
+        T* out = reinterpret_cast<T*>(p.out) + (size_t)at * p.n + even_column;
+        const T low = from_float<T>(first + bias[0]), high = from_float<T>(second + bias[1]);
+        if (words) {
+          *reinterpret_cast<uint32_t*>(out) = packed(low, high);
+        } else {
+          out[0] = low;
+          if (even_column + 1u < p.n) out[1] = high;
+        }
+      }
+    }
+  }
+}
+
+// Rows of x that a tile multiplies, its first weight row, and the output column of that row.
+struct Place {
+  uint32_t row, end, w_row, column;
+};
+template <uint32_t NT>
+__device__ __forceinline__ Place place_of(const Problem& p, uint32_t row_tile, uint32_t column) {
+  if (!p.plan.tiles) return {row_tile * NT, min(p.m, (row_tile + 1u) * NT), column, column};
+  const DenseTile rows = dense_tile(p.plan, row_tile);
+  const uint32_t row = min(rows.first, p.m), end = max(row, min(min(rows.end, p.m), row + kExpertTile));  // whatever the plan says
+  return {row, min(end, row + NT), min(rows.expert, p.plan.experts - 1u) * p.n + column, column};
+}
+// Bytes of the last word that lie behind k hold no exponents.
+__device__ __forceinline__ uint32_t last_word_mask(uint32_t k) {
+  return k % kWordValues ? (1u << (k % kWordValues / kBlock * 8u)) - 1u : 0xffffffffu;
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// Codes [rows, k / 2] read in boxes of 128 bytes x `box_rows` with the 128-byte swizzle; absent bytes read zero.
+inline bool make_map(CUtensorMap* map, const void* codes, uint64_t k, uint64_t rows, uint32_t box_rows) {
+  static EncodeTiled encode = []() -> EncodeTiled {
+    void* pointer = nullptr;
+    cudaDriverEntryPointQueryResult result;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &pointer, cudaEnableDefault, &result) != cudaSuccess ||
+        result != cudaDriverEntryPointSuccess)
+      return nullptr;
+    return reinterpret_cast<EncodeTiled>(pointer);
+  }();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[2] = {k / 2, rows}, strides[1] = {k / 2};
+  const cuuint32_t box[2] = {kRowBytes, box_rows}, element_strides[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+
+inline uint32_t most_plan_tiles(uint32_t slots, uint32_t experts) { return slots / kExpertTile + (slots < experts ? slots : experts); }
+
+// Few rows: every weight is read once and what counts is how fast (mxfp4_stream.cu).  Many: mxfp4_tiles.cu.  row_tiles: those of the
+// plan there can be.
+template <Store S> int run_stream(const KernelArgs& args, const Problem& p, uint32_t row_tiles);
+template <Store S> int run_tiles(const KernelArgs& args, const Problem& p, uint32_t row_tiles);
+
+}  // namespace mxfp4
+}  // namespace llmopt
