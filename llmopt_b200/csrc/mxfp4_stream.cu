@@ -1,10 +1,9 @@
 // Products of few MXFP4 rows with MXFP4 matrices: the stream of the weights is what they cost, n k 17 / 32 bytes.
 //
-// A CTA has one tile of 128 weight rows and all of k or, as one of a cluster, a share of it: four thread blocks of 192 threads live on an SM,
-// so that while one starts or stores the others stream.  Warp 0 brings the codes of 256 elements of k at a time by TMA
-// (128-byte swizzle); warps 2 to 5 bring the exponents, a word (128 elements) per thread and row, requested ahead in registers and laid
-// down in the order that tcgen05.cp spreads over tensor memory; one thread of warp 1 issues copies and products; then warps 2 to
-// 5 read the sums out.  CTAs of a cluster leave their sums in shared memory and each joins a share of the rows, in the order of k.
+// A CTA has one tile of 128 weight rows and all of k or, as one of a cluster, a share of it, in stages of 512 elements of k.  Warp 0 brings
+// the codes by TMA (128-byte swizzle); warps 2 to 5 bring the exponents, a warp per word (128 elements) of the stage, requested ahead in
+// registers and laid down in the order that tcgen05.cp spreads over tensor memory; one lane of warp 1 issues copies and products; then
+// warps 2 to 5 read the sums out.  CTAs of a cluster hand each row's sums to the one that joins them, in the order of k.
 //
 // While the kernel before still runs, the tile's weights are asked into L2: that changes nothing that anybody reads, whoever writes them.
 //
@@ -16,33 +15,48 @@ namespace llmopt {
 namespace {
 using namespace mxfp4;
 
-constexpr uint32_t kThreads = (2 + kScaleWarps) * 32, kAhead = 4, kMostSplits = 8;
+constexpr uint32_t kThreads = (2 + kScaleWarps) * 32, kMostSplits = 8, kMostShared = 227 * 1024;
+constexpr uint32_t kAhead = 4;               // stages of exponents that are under way in registers
+constexpr uint32_t kDepth = 512, kBoxes = kDepth / kBoxDepth, kStageWords = kDepth / kWordValues;
+static_assert(kStageWords == kScaleWarps, "a warp per word of a stage");
 
 template <uint32_t NT>
 struct Shape {
-  static constexpr uint32_t kWeightBytes = kColumns * kRowBytes, kInputBytes = NT * kRowBytes;
-  static constexpr uint32_t kScalesAt = kWeightBytes + kInputBytes;
-  static constexpr uint32_t kStageBytes = kScalesAt + kStageWords * 2 * kAtom;
-  static constexpr uint32_t kStages = 3;
-  static constexpr uint32_t kScaleColumns = kStageWords * 4 * 2;
+  static constexpr uint32_t kWeightBytes = kBoxes * kColumns * kRowBytes, kInputBytes = kBoxes * NT * kRowBytes;
+  static constexpr uint32_t kScalesAt = kWeightBytes + kInputBytes, kInputScalesAt = kScalesAt + kStageWords * kAtom;
+  static constexpr uint32_t kStageBytes = kInputScalesAt + kStageWords * kAtom;
+  static constexpr uint32_t kStages = 4;  // at most
+  static constexpr uint32_t kScaleColumns = kStageWords * 8;
   static constexpr uint32_t kUsedColumns = NT + 2 * kScaleColumns;
-  static constexpr uint32_t kTmemColumns = kUsedColumns <= 64 ? 64 : kUsedColumns <= 128 ? 128 : 256;
+  static constexpr uint32_t kTmemColumns = kUsedColumns <= 128 ? 128 : 256;
   static constexpr uint32_t kHolder = (3 * kStages + 1) * 8;  // behind the ring: barriers, tensor memory's address, abort flag
   static constexpr uint32_t kBehind = kHolder + 8;
   static constexpr uint32_t kPiece = NT == 16 ? 16 : 32;
-  // slack: 1024-byte alignment of the tiles; the ring holds the sums of a cluster's CTA afterwards
-  static constexpr __host__ __device__ uint32_t bytes(uint32_t stages) {
-    const uint32_t ring = stages * kStageBytes, sums = NT * kColumns * 4;
-    return (ring > sums ? ring : sums) + kBehind + 1024;
-  }
 };
 
 struct Work {
   uint32_t row_tiles, column_tiles, splits, stages, box_rows;
+  uint32_t share;  // rows that a CTA of a cluster joins
+  uint32_t parts;  // tiles here per tile of the plan
 };
+// Shared memory, 1024 of it for the alignment of the ring; behind the barriers the sums of a cluster's CTAs, [from][row of the share][column],
+// and a row that may be read but not used.
+template <uint32_t NT>
+uint32_t shared_bytes(const Work& work) {
+  using Z = Shape<NT>;
+  return 1024u + work.stages * Z::kStageBytes + Z::kBehind + (work.splits > 1u ? (work.splits * work.share + 1u) * kColumns * 4u : 0u);
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_store(uint32_t local, uint32_t rank, uint32_t value) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(remote), "r"(value) : "memory");
+}
 
 template <uint32_t NT, Store S>
-__global__ void __launch_bounds__(kThreads, NT <= 32 ? 3 : 2)
+__global__ void __launch_bounds__(kThreads, 2)
 stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Problem p, const Work work,
               uint32_t* error_word) {
   using Z = Shape<NT>;
@@ -50,67 +64,88 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
   grid_launch_dependents();
   const uint32_t base = (smem_u32(shared_raw) + 1023u) & ~1023u;
   unsigned char* base_pointer = shared_raw + (base - smem_u32(shared_raw));
-  const uint32_t behind = Z::bytes(work.stages) - Z::kBehind - 1024u;
+  const uint32_t behind = work.stages * Z::kStageBytes;
   const uint32_t full = base + behind, scales_full = full + Z::kStages * 8, empty = scales_full + Z::kStages * 8, sums_full = empty + Z::kStages * 8;
+  const uint32_t joined = base + behind + Z::kBehind;
   volatile uint32_t* holder = reinterpret_cast<volatile uint32_t*>(base_pointer + behind + Z::kHolder);
   volatile uint32_t* abort_flag = holder + 1;
-  const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u, t = threadIdx.x - 64u;  // t: row of the exponents' threads
+  const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u;
   const uint32_t splits = work.splits, rank = blockIdx.x % splits, tile = blockIdx.x / splits;
   const uint32_t column = tile / work.row_tiles * kColumns, k_stages = (p.k + kDepth - 1u) / kDepth;
   const uint32_t stage0 = k_stages * rank / splits, stage1 = k_stages * (rank + 1u) / splits, words = words_of(p.k);
 
-  if (threadIdx.x == 0) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
-    for (uint32_t s = 0; s < work.stages; ++s) {
-      barrier_init(full + s * 8, 1);  // the copies' expect_tx arrival; completes by byte count
-      barrier_init(scales_full + s * 8, kScaleWarps);
-      barrier_init(empty + s * 8, 1);  // one tcgen05.commit
+  if (warp == 0) {
+    if (lane == 0) {
+      for (uint32_t s = 0; s < work.stages; ++s) {
+        barrier_init(full + s * 8, 1);  // the copies' expect_tx arrival; completes by byte count
+        barrier_init(scales_full + s * 8, kScaleWarps);
+        barrier_init(empty + s * 8, 1);  // one tcgen05.commit
+      }
+      barrier_init(sums_full, 1);  // one tcgen05.commit
+      *abort_flag = 0u;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    barrier_init(sums_full, 1);  // one tcgen05.commit
-    *abort_flag = 0u;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (!p.plan.tiles)
-      for (uint32_t ks = stage0; ks < stage1; ++ks)
-        asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(&map_w), "r"((int32_t)(ks * kRowBytes)), "r"((int32_t)column)
+    __syncwarp();
+    if (!p.plan.tiles && elect_one())
+      for (uint32_t box = stage0 * kBoxes; box < stage1 * kBoxes && box * kBoxDepth < p.k; ++box)
+        asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(&map_w), "r"((int32_t)(box * kRowBytes)), "r"((int32_t)column)
                      : "memory");
+    __syncwarp();
   }
+  if (warp >= 2 && !p.plan.tiles)
+    for (uint32_t group = stage0 * kStageWords + warp - 2u; group < min(stage1 * kStageWords, words); group += kStageWords)
+      if (const uint32_t row = column + lane * 32u; lane < kColumns / 32u && row < p.w_rows)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.w_scales + (size_t)group * p.w_rows + row) : "memory");
+  if (splits > 1u) cluster_arrive();  // this CTA runs: others may write into its shared memory
   grid_dependency_wait();
-  if (p.plan.tiles && tile % work.row_tiles >= min(p.plan.tiles[0], work.row_tiles)) return;  // the whole cluster
-  const Place at = place_of<NT>(p, tile % work.row_tiles, column);
+  // whole clusters leave: those of tiles that the plan does not have, and of halves of its tiles without rows
+  if (p.plan.tiles && tile % work.row_tiles / work.parts >= min(p.plan.tiles[0], work.row_tiles / work.parts)) return;
+  const Place at = place_of<NT>(p, tile % work.row_tiles, work.parts, column);
+  if (p.plan.tiles && at.row >= at.end) return;
 
   auto give_up = [&]() {
     *abort_flag = 1u;
     if (error_word) atomicExch(error_word, 1u);
   };
-  const uint32_t boxes = (at.end - at.row + work.box_rows - 1u) / work.box_rows;
+  const uint32_t x_boxes = uniform((at.end - at.row + work.box_rows - 1u) / work.box_rows), w_row = uniform(at.w_row), x_row = uniform(at.row);
   auto load = [&](uint32_t ks, uint32_t s) {
-    const uint32_t stage = base + s * Z::kStageBytes;
-    barrier_expect_tx(full + s * 8, Z::kWeightBytes + boxes * work.box_rows * kRowBytes);
-    tma_load_2d(stage, &map_w, (int32_t)(ks * kRowBytes), (int32_t)at.w_row, full + s * 8);
-    for (uint32_t box = 0; box < boxes; ++box)
-      tma_load_2d(stage + Z::kWeightBytes + box * work.box_rows * kRowBytes, &map_x, (int32_t)(ks * kRowBytes), (int32_t)(at.row + box * work.box_rows),
-                  full + s * 8);
+    const uint32_t stage = base + s * Z::kStageBytes, boxes = min(kBoxes, (p.k - ks * kDepth + kBoxDepth - 1u) / kBoxDepth);
+    if (elect_one()) {
+      barrier_expect_tx(full + s * 8, boxes * (kColumns + x_boxes * work.box_rows) * kRowBytes);
+      for (uint32_t box = 0; box < boxes; ++box) {
+        const int32_t x = (int32_t)((ks * kBoxes + box) * kRowBytes);
+        tma_load_2d(stage + box * kColumns * kRowBytes, &map_w, x, (int32_t)w_row, full + s * 8);
+        for (uint32_t i = 0; i < x_boxes; ++i)
+          tma_load_2d(stage + Z::kWeightBytes + (box * NT + i * work.box_rows) * kRowBytes, &map_x, x, (int32_t)(x_row + i * work.box_rows), full + s * 8);
+      }
+    }
+    __syncwarp();
   };
-  // words of the weights and of x, a stage each; nothing looks at them before they are laid down, so that nothing waits for them here
-  uint32_t held[kAhead][kStageWords * 2];
-  auto fetch = [&](uint32_t ks, uint32_t (&into)[kStageWords * 2]) {
+  // The words of group warp - 2 of a stage: of the weight rows lane, lane + 32, ..., and of as many rows of x.  Nothing looks at them before
+  // they are laid down, so that nothing waits for them here.
+  constexpr uint32_t kInputWords = NT <= 32 ? 1 : NT / 32;
+  uint32_t held[kAhead][4 + kInputWords];
+  auto fetch = [&](uint32_t ks, uint32_t (&into)[4 + kInputWords]) {
+    const uint32_t group = ks * kStageWords + warp - 2u;
+    const bool present = ks < stage1 && group < words;
 #pragma unroll
-    for (uint32_t g = 0; g < kStageWords; ++g) {
-      const uint32_t group = ks * kStageWords + g;
-      const bool present = ks < stage1 && group < words;
-      into[2 * g] = into[2 * g + 1] = 0u;
-      if (present && at.w_row + t < p.w_rows) into[2 * g] = p.w_scales[(size_t)group * p.w_rows + at.w_row + t];
-      if (present && t < NT && at.row + t < at.end) into[2 * g + 1] = p.x_scales[(size_t)group * p.m + at.row + t];
+    for (uint32_t i = 0; i < 4; ++i) {
+      into[i] = 0u;
+      if (present && at.w_row + i * 32u + lane < p.w_rows) into[i] = p.w_scales[(size_t)group * p.w_rows + at.w_row + i * 32u + lane];
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kInputWords; ++i) {
+      into[4 + i] = 0u;
+      if (present && at.row + i * 32u + lane < at.end) into[4 + i] = p.x_scales[(size_t)group * p.m + at.row + i * 32u + lane];
     }
   };
-  // ahead of the block's first synchronisation: the barriers are this thread's own, the words lie in registers
-  if (threadIdx.x == 0) {
+  // ahead of the block's first synchronisation: the barriers are this warp's own, the words lie in registers
+  if (warp == 0) {
     for (uint32_t s = 0; s < work.stages && stage0 + s < stage1; ++s) load(stage0 + s, s);
   } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + behind + Z::kHolder), "r"(Z::kTmemColumns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  } else if (warp >= 2) {
+  } else {
 #pragma unroll
     for (uint32_t a = 0; a < kAhead; ++a) fetch(stage0 + a, held[a]);
   }
@@ -129,8 +164,7 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         give_up();
         break;
       }
-      if (elect_one()) load(ks, s);
-      __syncwarp();
+      load(ks, s);
       if (++s == work.stages) s = 0, phase ^= 1u;
     }
     // on the way out after a failure the copies already started must land first
@@ -149,20 +183,21 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t scales = tmem_base + NT + (ks & 1u) * Z::kScaleColumns, left = p.k - ks * kDepth;
+      const uint32_t scales = tmem_base + NT + (ks & 1u) * Z::kScaleColumns, x_scales = scales + kStageWords * 4u, left = p.k - ks * kDepth;
       const uint64_t a = operand_descriptor(stage), b = operand_descriptor(stage + Z::kWeightBytes);
       if (elect_one()) {
 #pragma unroll
         for (uint32_t g = 0; g < kStageWords; ++g) {
           if (g * kWordValues >= left) break;
-          copy_atom(scales + g * 8u, stage + Z::kScalesAt + 2u * g * kAtom);
-          copy_atom(scales + g * 8u + 4u, stage + Z::kScalesAt + (2u * g + 1u) * kAtom);
-        }
+          copy_atom(scales + g * 4u, stage + Z::kScalesAt + g * kAtom);
+          copy_atom(x_scales + g * 4u, stage + Z::kInputScalesAt + g * kAtom);
 #pragma unroll
-        for (uint32_t j = 0; j < kDepth / 64; ++j) {
-          if (j * 64u >= left) break;
-          const uint32_t columns = scales + j / 2u * 8u;
-          mma_mxf4(tmem_base, a + j * 2u, b + j * 2u, j & 1u ? high : low, columns, columns + 4u, (ks > stage0 || j > 0) ? 1u : 0u);
+          for (uint32_t j = 0; j < 2; ++j) {
+            if (g * kWordValues + j * 64u >= left) break;
+            const uint32_t box = g / 2u, at_box = (g % 2u * 2u + j) * 2u;  // 32 bytes of the box's rows, in the descriptor's 16
+            mma_mxf4(tmem_base, a + box * (kColumns * kRowBytes / 16u) + at_box, b + box * (NT * kRowBytes / 16u) + at_box, j ? high : low,
+                     scales + g * 4u, x_scales + g * 4u, (ks > stage0 || g > 0 || j > 0) ? 1u : 0u);
+          }
         }
         mma_commit(empty + s * 8);
         if (ks + 1u == stage1) mma_commit(sums_full);
@@ -172,7 +207,7 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     }
     if (!ok) give_up();
   } else {
-    const uint32_t target = (t & 31u) * 16u + (t >> 5) * 4u, last_mask = last_word_mask(p.k);  // a row's place in an atom
+    const uint32_t group = warp - 2u, last_mask = last_word_mask(p.k);
     bool ok = true;
     uint32_t s = 0, phase = 1;
     for (uint32_t first = stage0; first < stage1 && ok; first += kAhead) {
@@ -180,13 +215,17 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
       for (uint32_t a = 0; a < kAhead; ++a) {
         const uint32_t ks = first + a;
         if (ks >= stage1 || !ok) break;
-        ok = !*abort_flag && barrier_wait(empty + s * 8, phase);
+        ok = !*abort_flag && warp_wait(empty + s * 8, phase);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        unsigned char* atoms = base_pointer + s * Z::kStageBytes + Z::kScalesAt + target;
+        const uint32_t mask = ks * kStageWords + group + 1u == words ? last_mask : 0xffffffffu;
+        unsigned char* const stage = base_pointer + s * Z::kStageBytes;
+        // a lane's four rows are a line of the atom
+        *reinterpret_cast<uint4*>(stage + Z::kScalesAt + group * kAtom + lane * 16u) =
+            make_uint4(held[a][0] & mask, held[a][1] & mask, held[a][2] & mask, held[a][3] & mask);
 #pragma unroll
-        for (uint32_t w = 0; w < kStageWords * 2; ++w)
-          *reinterpret_cast<uint32_t*>(atoms + w * kAtom) = held[a][w] & (ks * kStageWords + w / 2 + 1u == words ? last_mask : 0xffffffffu);
+        for (uint32_t i = 0; i < kInputWords; ++i)
+          *reinterpret_cast<uint32_t*>(stage + Z::kInputScalesAt + group * kAtom + lane * 16u + i * 4u) = held[a][4 + i] & mask;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) barrier_arrive(scales_full + s * 8);
@@ -195,14 +234,16 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
       }
     }
     if (ok) {
-      ok = !*abort_flag && barrier_wait(sums_full, 0u);
+      ok = !*abort_flag && warp_wait(sums_full, 0u);
       ok = __all_sync(0xffffffffu, ok);
     }
+    if (splits > 1u) cluster_wait();
     if (!ok) {
       give_up();
     } else {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t quarter = warp & 3u, address = tmem_base + ((quarter * 32u) << 16);
+      const uint32_t quarter = warp & 3u, address = tmem_base + ((quarter * 32u) << 16), place = quarter * 32u + lane;
+      uint32_t owner = 0, share_row = 0;
 #pragma unroll 1
       for (uint32_t piece = 0; piece < NT / Z::kPiece; ++piece) {
         const uint32_t row = at.row + piece * Z::kPiece;
@@ -212,74 +253,77 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         else tmem_load_32(address + piece * Z::kPiece, raw);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         if (splits == 1u) {
-          store_rows<S>(p, row, at.end, at.column + quarter * 32u + lane, raw);
+          store_rows<S>(p, row, at.end, at.column + place, raw);
         } else {
-          // [row][column] of the partial sums, over the ring: every stage of it has been read
-          float* partial = reinterpret_cast<float*>(base_pointer) + piece * Z::kPiece * kColumns + quarter * 32u + lane;
 #pragma unroll
-          for (uint32_t i = 0; i < Z::kPiece; ++i) partial[i * kColumns] = __uint_as_float(raw[i]);
+          for (uint32_t i = 0; i < Z::kPiece; ++i) {
+            if (row + i >= at.end) break;
+            cluster_store(joined + ((rank * work.share + share_row) * kColumns + place) * 4u, owner, raw[i]);
+            if (++share_row == work.share) share_row = 0, ++owner;
+          }
         }
         __syncwarp();  // tcgen05.ld needs the whole warp
       }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
+  if (warp < 2u && splits > 1u) cluster_wait();
 
   __syncthreads();
-  // Before CTAs of a cluster wait for one another: one that waits for columns which another grid holds must not be waited for with these held.
+  // Before CTAs of a cluster wait for one another's sums: one that waits for columns which another grid holds must not be waited for with
+  // these held.
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Z::kTmemColumns) : "memory");
   }
   if (splits == 1u) return;
-  cluster_sync();
-  // each CTA joins a share of the rows, always the partial sums of rank 0 first; a warp has 32 columns of two rows at a time
-  const float* partial = reinterpret_cast<const float*>(base_pointer);
-  const uint32_t pairs = (at.end - at.row + 1u) / 2u;
-  for (uint32_t item = rank * (kThreads / 32u) + warp; item < pairs * 4u; item += splits * (kThreads / 32u)) {
+  cluster_arrive();
+  cluster_wait();
+  // this CTA's share of the rows, always the sums of rank 0 first; a warp has 32 columns of two rows at a time
+  const float* sums = reinterpret_cast<const float*>(base_pointer + behind + Z::kBehind);
+  const uint32_t first_row = rank * work.share, all = at.end - at.row, mine = first_row < all ? min(work.share, all - first_row) : 0u;
+  for (uint32_t item = warp; item < (mine + 1u) / 2u * 4u; item += kThreads / 32u) {
     const uint32_t row = item / 4u * 2u, place = item % 4u * 32u + lane;
-    float part[2][kMostSplits];
-#pragma unroll
-    for (uint32_t from = 0; from < kMostSplits; ++from)
-#pragma unroll
-      for (uint32_t i = 0; i < 2; ++i) part[i][from] = from < splits ? cluster_load(partial + (row + i) * kColumns + place, from) : 0.0f;
     uint32_t raw[2];
 #pragma unroll
     for (uint32_t i = 0; i < 2; ++i) {
-      float sum = part[i][0];
-#pragma unroll
-      for (uint32_t from = 1; from < kMostSplits; ++from)
-        if (from < splits) sum += part[i][from];
+      float sum = sums[(row + i) * kColumns + place];
+      for (uint32_t from = 1; from < splits; ++from) sum += sums[(from * work.share + row + i) * kColumns + place];
       raw[i] = __float_as_uint(sum);
     }
-    store_rows<S>(p, at.row + row, at.end, at.column + place, raw);
+    store_rows<S>(p, at.row + first_row + row, at.row + first_row + mine, at.column + place, raw);
   }
-  cluster_sync();  // nobody leaves while its sums are read
 }
 
 template <uint32_t NT, Store S>
 int run(const KernelArgs& args, const Problem& p, uint32_t row_tiles) {
   using Z = Shape<NT>;
   const uint32_t sms = (uint32_t)context_sm_count(args.ctx), k_stages = (p.k + kDepth - 1u) / kDepth;
-  Work work = {row_tiles, (p.n + kColumns - 1u) / kColumns, 1u, 0u, p.plan.tiles ? 16u : NT};
+  Work work = {row_tiles, (p.n + kColumns - 1u) / kColumns, 1u, 0u, p.plan.tiles ? 16u : NT, 0u, NT == 64 && p.m > 64u ? kExpertTile / 64u : 1u};
   const size_t tiles = (size_t)work.row_tiles * work.column_tiles;
   LLMOPT_REQUIRE(tiles < (1u << 28), "too many tiles");
-  // CTAs that share a tile's k while the tiles leave SMs without work
-  while (work.splits < kMostSplits && tiles * work.splits < 2u * (size_t)sms && k_stages >= work.splits * 4u) work.splits *= 2u;
+  // CTAs that share a tile's k while tiles leave SMs without work; powers of two, which leave the fewest SMs of a GPC over.  us with 1, 2, 4, 8
+  // of them: 4096 x 4096 6.3, 5.2, 4.3, 6.3; k 14336 x 4096 16.8, 11.5, 9.1, 18; 4096 x 14336 (112 tiles) 8.1, 12.
+  while (work.splits < kMostSplits && tiles * work.splits * 2u <= sms && k_stages >= work.splits * 2u) work.splits *= 2u;
   const uint32_t mine = (k_stages + work.splits - 1u) / work.splits;
-  work.stages = mine < Z::kStages ? mine : Z::kStages;
+  // a CTA per SM: a deep ring; more: two of them per SM, which start and end beside one another (4 and 2 stages: 4096 x 14336 8.1, 10.1 us;
+  // 4096 x 128256 57.9, 54.1)
+  const uint32_t most = tiles * work.splits <= sms ? Z::kStages : 2u;
+  work.stages = mine < most ? mine : most;
+  const uint32_t rows = p.m < NT ? p.m : NT;
+  work.share = (rows + work.splits - 1u) / work.splits;
   CUtensorMap map_w, map_x;
   LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.box_rows), "tensor map was refused");
   auto kernel = stream_kernel<NT, S>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::bytes(Z::kStages)) != cudaSuccess) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess) {
     cudaGetLastError();
     return fail(args, "shared memory request was refused");
   }
   const dim3 grid((uint32_t)tiles * work.splits);
   if (work.splits == 1u)
-    launch_kernel(args, kernel, grid, dim3(kThreads), Z::bytes(work.stages), map_w, map_x, p, work, context_device_error(args.ctx));
+    launch_kernel(args, kernel, grid, dim3(kThreads), shared_bytes<NT>(work), map_w, map_x, p, work, context_device_error(args.ctx));
   else
-    launch_cluster_kernel(args, kernel, grid, dim3(kThreads), Z::bytes(work.stages), work.splits, map_w, map_x, p, work,
+    launch_cluster_kernel(args, kernel, grid, dim3(kThreads), shared_bytes<NT>(work), work.splits, map_w, map_x, p, work,
                           context_device_error(args.ctx));
   return check_launch(args);
 }
@@ -290,11 +334,10 @@ namespace mxfp4 {
 
 template <Store S>
 int run_stream(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
-  const uint32_t row_tiles = p.plan.tiles ? plan_tiles : 1u;
-  if (p.m <= 16u) return run<16, S>(args, p, row_tiles);
-  if (p.m <= 32u) return run<32, S>(args, p, row_tiles);
-  if (p.m <= 64u) return run<64, S>(args, p, row_tiles);
-  return run<128, S>(args, p, row_tiles);
+  if (p.m <= 16u) return run<16, S>(args, p, p.plan.tiles ? plan_tiles : 1u);
+  if (p.m <= 32u) return run<32, S>(args, p, p.plan.tiles ? plan_tiles : 1u);
+  // a tile of the plan is up to two of these, most often one
+  return run<64, S>(args, p, p.plan.tiles ? plan_tiles * (p.m <= 64u ? 1u : kExpertTile / 64u) : 1u);
 }
 
 template int run_stream<kStoreHalf>(const KernelArgs&, const Problem&, uint32_t);

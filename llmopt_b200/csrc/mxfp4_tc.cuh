@@ -17,8 +17,9 @@ uint32_t* context_device_error(Context* ctx);
 namespace mxfp4 {
 using namespace tc;
 
-constexpr uint32_t kColumns = 128, kDepth = 256, kRowBytes = kDepth / 2;  // weight rows of a tile, elements of k of a stage
-constexpr uint32_t kStageWords = kDepth / kWordValues, kAtom = 512;       // an atom: the words of 128 rows
+constexpr uint32_t kColumns = 128;                                        // weight rows of a tile
+constexpr uint32_t kBoxDepth = 256, kRowBytes = kBoxDepth / 2;            // elements of k of a box of codes
+constexpr uint32_t kAtom = 512;                                           // an atom: the words of 128 rows
 constexpr uint32_t kScaleWarps = 4;  // a thread per weight row
 
 // One lane of a converged warp.  What the tensor cores and copies take lies in uniform registers: where the whole warp walks through a loop
@@ -111,12 +112,14 @@ __device__ __forceinline__ void store_rows(const Problem& p, uint32_t row, uint3
 struct Place {
   uint32_t row, end, w_row, column;
 };
+// A tile of the plan is `parts` tiles here.
 template <uint32_t NT>
-__device__ __forceinline__ Place place_of(const Problem& p, uint32_t row_tile, uint32_t column) {
+__device__ __forceinline__ Place place_of(const Problem& p, uint32_t row_tile, uint32_t parts, uint32_t column) {
   if (!p.plan.tiles) return {row_tile * NT, min(p.m, (row_tile + 1u) * NT), column, column};
-  const DenseTile rows = dense_tile(p.plan, row_tile);
-  const uint32_t row = min(rows.first, p.m), end = max(row, min(min(rows.end, p.m), row + kExpertTile));  // whatever the plan says
-  return {row, min(end, row + NT), min(rows.expert, p.plan.experts - 1u) * p.n + column, column};
+  const DenseTile rows = dense_tile(p.plan, row_tile / parts);
+  const uint32_t first = min(rows.first, p.m), last = max(first, min(min(rows.end, p.m), first + kExpertTile));  // whatever the plan says
+  const uint32_t row = min(first + row_tile % parts * NT, last);
+  return {row, min(last, row + NT), min(rows.expert, p.plan.experts - 1u) * p.n + column, column};
 }
 // Bytes of the last word that lie behind k hold no exponents.
 __device__ __forceinline__ uint32_t last_word_mask(uint32_t k) {

@@ -12,7 +12,7 @@ namespace llmopt {
 namespace {
 using namespace mxfp4;
 
-constexpr uint32_t kAhead = 4;
+constexpr uint32_t kAhead = 4, kDepth = kBoxDepth, kStageWords = kDepth / kWordValues;  // of a stage
 
 template <uint32_t NT>
 struct Shape {
@@ -54,7 +54,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u;
   const uint32_t row_tiles = p.plan.tiles ? min(p.plan.tiles[0], work.row_tiles) : work.row_tiles;
   const uint32_t tiles = row_tiles * work.column_tiles, k_stages = (p.k + kDepth - 1u) / kDepth;
-  auto place = [&](uint32_t tile) { return place_of<NT>(p, tile % row_tiles, tile / row_tiles * kColumns); };
+  auto place = [&](uint32_t tile) { return place_of<NT>(p, tile % row_tiles, 1u, tile / row_tiles * kColumns); };
 
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < Z::kStages; ++s) {
