@@ -37,7 +37,7 @@ struct Shape {
 struct Work {
   uint32_t row_tiles, column_tiles, splits, stages, box_rows;
   uint32_t share;  // rows that a CTA of a cluster joins
-  uint32_t parts;  // tiles here per tile of the plan
+  uint32_t parts;  // tiles here per tile of the plan, most often one of which has rows
 };
 // Shared memory, 1024 of it for the alignment of the ring; behind the barriers the sums of a cluster's CTAs, [from][row of the share][column],
 // and a row that may be read but not used.
@@ -100,7 +100,7 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
   grid_dependency_wait();
   // whole clusters leave: those of tiles that the plan does not have, and of halves of its tiles without rows
   if (p.plan.tiles && tile % work.row_tiles / work.parts >= min(p.plan.tiles[0], work.row_tiles / work.parts)) return;
-  const Place at = place_of<NT>(p, tile % work.row_tiles, work.parts, column);
+  const Place at = place_of(p, tile % work.row_tiles, NT, work.parts, column);
   if (p.plan.tiles && at.row >= at.end) return;
 
   auto give_up = [&]() {
@@ -174,7 +174,7 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     __syncwarp();
   } else if (warp == 1) {
     const uint32_t rows = p.plan.tiles ? uniform(max((at.end - at.row + 15u) / 16u * 16u, 16u)) : NT;
-    const uint32_t low = mxf4_instruction(rows, 0u), high = mxf4_instruction(rows, 1u);
+    const uint32_t low = mxf4_instruction(kColumns, rows, 0u), high = mxf4_instruction(kColumns, rows, 1u);
     bool ok = true;
     uint32_t s = 0, phase = 0;
     for (uint32_t ks = stage0; ks < stage1; ++ks) {
@@ -296,10 +296,11 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 }
 
 template <uint32_t NT, Store S>
-int run(const KernelArgs& args, const Problem& p, uint32_t row_tiles) {
+int run(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
   using Z = Shape<NT>;
   const uint32_t sms = (uint32_t)context_sm_count(args.ctx), k_stages = (p.k + kDepth - 1u) / kDepth;
-  Work work = {row_tiles, (p.n + kColumns - 1u) / kColumns, 1u, 0u, p.plan.tiles ? 16u : NT, 0u, NT == 64 && p.m > 64u ? kExpertTile / 64u : 1u};
+  const uint32_t parts = p.m <= NT ? 1u : kExpertTile / NT;
+  Work work = {p.plan.tiles ? plan_tiles * parts : 1u, (p.n + kColumns - 1u) / kColumns, 1u, 0u, p.plan.tiles ? 16u : NT, 0u, parts};
   const size_t tiles = (size_t)work.row_tiles * work.column_tiles;
   LLMOPT_REQUIRE(tiles < (1u << 28), "too many tiles");
   // CTAs that share a tile's k while tiles leave SMs without work; powers of two, which leave the fewest SMs of a GPC over.  us with 1, 2, 4, 8
@@ -315,10 +316,7 @@ int run(const KernelArgs& args, const Problem& p, uint32_t row_tiles) {
   CUtensorMap map_w, map_x;
   LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.box_rows), "tensor map was refused");
   auto kernel = stream_kernel<NT, S>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess) {
-    cudaGetLastError();
-    return fail(args, "shared memory request was refused");
-  }
+  LLMOPT_REQUIRE((allow_shared<kMostShared, stream_kernel<NT, S>>()), "shared memory request was refused");
   const dim3 grid((uint32_t)tiles * work.splits);
   if (work.splits == 1u)
     launch_kernel(args, kernel, grid, dim3(kThreads), shared_bytes<NT>(work), map_w, map_x, p, work, context_device_error(args.ctx));
@@ -334,10 +332,9 @@ namespace mxfp4 {
 
 template <Store S>
 int run_stream(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
-  if (p.m <= 16u) return run<16, S>(args, p, p.plan.tiles ? plan_tiles : 1u);
-  if (p.m <= 32u) return run<32, S>(args, p, p.plan.tiles ? plan_tiles : 1u);
-  // a tile of the plan is up to two of these, most often one
-  return run<64, S>(args, p, p.plan.tiles ? plan_tiles * (p.m <= 64u ? 1u : kExpertTile / 64u) : 1u);
+  if (p.m <= 16u) return run<16, S>(args, p, plan_tiles);
+  if (p.m <= 32u) return run<32, S>(args, p, plan_tiles);
+  return run<64, S>(args, p, plan_tiles);
 }
 
 template int run_stream<kStoreHalf>(const KernelArgs&, const Problem&, uint32_t);

@@ -7,6 +7,8 @@
 #pragma once
 #include <cuda.h>
 
+#include <atomic>
+
 #include "mxfp4.cuh"
 #include "w4a16_tc_device.cuh"
 
@@ -34,8 +36,8 @@ __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xf
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, barrier_wait(bar, parity)); }
 
 // kind::mxf4, e2m1 A and B (format 1), e8m0 scales, both K-major; `pair` picks the half of a scale word.
-__device__ __forceinline__ uint32_t mxf4_instruction(uint32_t n, uint32_t pair) {
-  return (pair << 5) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((kColumns >> 4) << 24) | (pair << 30);
+__device__ __forceinline__ uint32_t mxf4_instruction(uint32_t m, uint32_t n, uint32_t pair) {
+  return (pair << 5) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 4) << 24) | (pair << 30);
 }
 __device__ __forceinline__ void mma_mxf4(uint32_t sums, uint64_t a, uint64_t b, uint32_t instruction, uint32_t a_scales, uint32_t b_scales,
                                          uint32_t accumulate) {
@@ -46,11 +48,14 @@ __device__ __forceinline__ void mma_mxf4(uint32_t sums, uint64_t a, uint64_t b, 
       ::"r"(sums), "l"(a), "l"(b), "r"(instruction), "r"(accumulate), "r"(a_scales), "r"(b_scales)
       : "memory");
 }
-// An atom (32 rows of 16 bytes, unswizzled, eight rows every 128 bytes) to four columns, the same in all four quarters of the lanes.
-__device__ __forceinline__ void copy_atom(uint32_t columns, uint32_t shared_address) {
+// An atom (32 rows of 16 bytes, unswizzled, eight rows every 128 bytes) to four columns, the same in all four quarters of the lanes.  Scale
+// operands start at multiples of four columns.
+__device__ __forceinline__ uint64_t atom_descriptor(uint32_t shared_address) {
   constexpr uint64_t kForm = (uint64_t)(128 >> 4) << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
-  const uint64_t descriptor = kForm | (uint64_t)((shared_address & 0x3ffffu) >> 4);
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(columns), "l"(descriptor) : "memory");
+  return kForm | (uint64_t)((shared_address & 0x3ffffu) >> 4);
+}
+__device__ __forceinline__ void copy_atom(uint32_t columns, uint32_t shared_address) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(columns), "l"(atom_descriptor(shared_address)) : "memory");
 }
 
 enum Store : uint32_t { kStoreHalf, kStoreBf16, kStoreFloat, kStorePairHalf, kStorePairBf16 };
@@ -112,14 +117,13 @@ __device__ __forceinline__ void store_rows(const Problem& p, uint32_t row, uint3
 struct Place {
   uint32_t row, end, w_row, column;
 };
-// A tile of the plan is `parts` tiles here.
-template <uint32_t NT>
-__device__ __forceinline__ Place place_of(const Problem& p, uint32_t row_tile, uint32_t parts, uint32_t column) {
-  if (!p.plan.tiles) return {row_tile * NT, min(p.m, (row_tile + 1u) * NT), column, column};
-  const DenseTile rows = dense_tile(p.plan, row_tile / parts);
-  const uint32_t first = min(rows.first, p.m), last = max(first, min(min(rows.end, p.m), first + kExpertTile));  // whatever the plan says
-  const uint32_t row = min(first + row_tile % parts * NT, last);
-  return {row, min(last, row + NT), min(rows.expert, p.plan.experts - 1u) * p.n + column, column};
+// Tiles have at most `rows` rows; one of the plan is `parts` of them.
+__device__ __forceinline__ Place place_of(const Problem& p, uint32_t row_tile, uint32_t rows, uint32_t parts, uint32_t column) {
+  if (!p.plan.tiles) return {row_tile * rows, min(p.m, (row_tile + 1u) * rows), column, column};
+  const DenseTile tile = dense_tile(p.plan, row_tile / parts);
+  const uint32_t first = min(tile.first, p.m), last = max(first, min(min(tile.end, p.m), first + kExpertTile));  // whatever the plan says
+  const uint32_t row = min(first + row_tile % parts * rows, last);
+  return {row, min(last, row + rows), min(tile.expert, p.plan.experts - 1u) * p.n + column, column};
 }
 // Bytes of the last word that lie behind k hold no exponents.
 __device__ __forceinline__ uint32_t last_word_mask(uint32_t k) {
@@ -146,6 +150,22 @@ inline bool make_map(CUtensorMap* map, const void* codes, uint64_t k, uint64_t r
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+
+// Lets a kernel have BYTES of shared memory, the most that any launch of it asks for; said once per device.
+template <uint32_t BYTES, auto KERNEL>
+bool allow_shared() {
+  static std::atomic<uint64_t> said{0};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  const uint64_t bit = (uint64_t)1 << (device & 63);
+  if (said.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  said.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
 
 inline uint32_t most_plan_tiles(uint32_t slots, uint32_t experts) { return slots / kExpertTile + (slots < experts ? slots : experts); }
 

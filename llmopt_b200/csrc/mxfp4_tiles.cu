@@ -1,11 +1,16 @@
-// Products of many MXFP4 rows: persistent CTAs walk over tiles of 128 weight rows by 128 or 256 rows of x.
+// Products of many MXFP4 rows: pairs of CTAs walk over tiles of 256 weight rows by up to 224 rows of x.
 //
-// A CTA: warp 0 brings the codes of 256 elements of k of 128 weight rows and of the tile's rows of x by TMA (128-byte swizzle); warps 2 to 5
-// bring their exponents, a word (128 elements) per thread and row, requested four stages ahead and laid down in the order that tcgen05.cp
-// spreads over tensor memory; one thread of warp 1 issues copies and products; the other warps read the sums out.
+// What bounds a tile is how often its operands come from L2: tcgen05.mma with cta_group::2 multiplies 256 weight rows, half of them in
+// either CTA's shared memory, with rows of x of which either CTA holds half as well, 30 KB for what a CTA by itself needs 44 KB for.
+// In each CTA warp 0 brings the codes of 256 elements of k of its halves by TMA (128-byte swizzle); warps 2 and 3 bring the exponents of
+// its 128 weight rows, warps 4 and 5 those of all rows of x, a warp per word of a stage, requested four stages ahead and laid down
+// in the order that tcgen05.cp spreads over tensor memory.  One lane of warp 1 of the first CTA issues copies and products for
+// both, and its barriers count both CTAs' copies and exponents.  Eight more warps read a tile's sums out, each a quarter of the
+// lanes (output columns), while the next tile's are formed in other columns of tensor memory; results of 16 bits change
+// places in shared memory, so that four lanes share 64 bytes of a row.
 //
-// Every wait on an mbarrier is bounded; a wait that runs out raises the context's device error word, and the CTA lets its copies land,
-// frees its tensor memory and returns.
+// Every wait on an mbarrier is bounded; a wait that runs out raises the context's device error word, and the CTA lets its copies and
+// products end, frees its tensor memory and returns.
 #include "mxfp4_tc.cuh"
 
 namespace llmopt {
@@ -13,68 +18,144 @@ namespace {
 using namespace mxfp4;
 
 constexpr uint32_t kAhead = 4, kDepth = kBoxDepth, kStageWords = kDepth / kWordValues;  // of a stage
-
-template <uint32_t NT>
-struct Shape {
-  static constexpr uint32_t kAtoms = (NT + 127) / 128;  // of x, per word
-  static constexpr uint32_t kWeightBytes = kColumns * kRowBytes, kInputBytes = NT * kRowBytes;
-  static constexpr uint32_t kScalesAt = kWeightBytes + kInputBytes;
-  static constexpr uint32_t kStageBytes = kScalesAt + kStageWords * (1 + kAtoms) * kAtom;
-  static constexpr uint32_t kStages = NT == 256 ? 4 : 6;
-  static constexpr uint32_t kSums = NT == 256 ? 1 : 2;  // accumulators
-  static constexpr uint32_t kScaleColumns = kStageWords * 4 * (1 + kAtoms);
-  static constexpr uint32_t kUsedColumns = kSums * NT + 2 * kScaleColumns;
-  static constexpr uint32_t kTmemColumns = 512;
-  static_assert(kUsedColumns <= kTmemColumns, "tensor memory");
-  static constexpr uint32_t kBarriers = kStages * kStageBytes;
-  static constexpr uint32_t kHolder = kBarriers + (3 * kStages + 4) * 8;
-  static constexpr uint32_t kAbort = kHolder + 4;
-  static constexpr uint32_t kSharedBytes = kAbort + 4 + 1024;  // slack: 1024-byte alignment of the tiles
-  static constexpr uint32_t kEpilogueWarps = 8;
-  static constexpr uint32_t kThreads = (2 + kScaleWarps + kEpilogueWarps) * 32;
-};
+constexpr uint32_t kMostRows = 224, kInputAtoms = 2;
+constexpr uint32_t kEpilogueWarps = 8, kThreads = (2 + kScaleWarps + kEpilogueWarps) * 32;
+constexpr uint32_t kWeightBytes = kColumns * kRowBytes, kInputBytes = kMostRows / 2 * kRowBytes;
+constexpr uint32_t kScalesAt = kWeightBytes + kInputBytes, kInputScalesAt = kScalesAt + kStageWords * kAtom;
+constexpr uint32_t kStageBytes = kInputScalesAt + kStageWords * kInputAtoms * kAtom;
+constexpr uint32_t kStages = 6, kSums = 2;
+constexpr uint32_t kScaleColumns = kStageWords * 4 * (1 + kInputAtoms), kTmemColumns = 512;
+static_assert(kSums * kMostRows + 2 * kScaleColumns <= kTmemColumns && kStageBytes % 1024 == 0, "tensor memory, alignment of tiles");
+constexpr uint32_t kStagingRow = 80, kStagingBytes = 32 * kStagingRow;  // a warp's 32 rows of 64 bytes and 16 of padding
+constexpr uint32_t kStaging = kStages * kStageBytes, kBarriers = kStaging + kEpilogueWarps * kStagingBytes;
+constexpr uint32_t kHolder = kBarriers + (3 * kStages + 2 * kSums + 1) * 8, kAbort = kHolder + 4;
+constexpr uint32_t kSharedBytes = kAbort + 4 + 1024;  // slack: 1024-byte alignment of the tiles
+static_assert(kSharedBytes <= 227 * 1024, "shared memory");
 
 struct Work {
-  uint32_t row_tiles, column_tiles, box_rows;
+  uint32_t row_tiles, column_tiles;  // of x, of pairs of weight tiles
+  uint32_t rows, box_rows;           // most rows of a tile; rows of a box of x
 };
 
-template <uint32_t NT, Store S>
-__global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
-product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Problem p,
-               const Work work, uint32_t* error_word) {
-  using Z = Shape<NT>;
+// The first CTA's barriers, from either.
+__device__ __forceinline__ uint32_t first_address(uint32_t local) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(0u));
+  return remote;
+}
+__device__ __forceinline__ void first_arrive(uint32_t first) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(first) : "memory"); }
+// A tile to this CTA's shared memory whose bytes the barrier of the first one counts.
+__device__ __forceinline__ void pair_load(uint32_t destination, const CUtensorMap* map, int32_t x, int32_t y, uint32_t first) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(destination), "l"(map), "r"(first), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void pair_mma(uint32_t sums, uint64_t a, uint64_t b, uint32_t instruction, uint32_t a_scales, uint32_t b_scales,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+      ::"r"(sums), "l"(a), "l"(b), "r"(instruction), "r"(accumulate), "r"(a_scales), "r"(b_scales)
+      : "memory");
+}
+__device__ __forceinline__ void pair_copy_atom(uint32_t columns, uint32_t shared_address) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(columns), "l"(atom_descriptor(shared_address)) : "memory");
+}
+// arrives on both CTAs' barriers
+__device__ __forceinline__ void pair_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+               : "memory");
+}
+
+// 32 rows of sums of this lane's column, on their way out through the warp's staging.
+template <Store S>
+__device__ __forceinline__ void store_piece(const Problem& p, uint32_t row, uint32_t end, uint32_t column0, const uint32_t (&raw)[32], unsigned char* staging) {
+  typedef typename Element<S>::Type T;
+  constexpr bool kPair = S == kStorePairHalf || S == kStorePairBf16;
+  const uint32_t lane = threadIdx.x & 31u;
+  if constexpr (S == kStoreFloat) {
+    store_rows<S>(p, row, end, column0 + lane, raw);
+  } else {
+    if constexpr (kPair) {
+      const bool odd = lane & 1u;
+#pragma unroll
+      for (uint32_t i = 0; i < 32; i += 2) {
+        const uint32_t away = __shfl_xor_sync(0xffffffffu, odd ? raw[i] : raw[i + 1], 1), at = i + (odd ? 1u : 0u);
+        const float scale = row + at < end ? p.row_scale[row + at] : 0.0f;
+        const float gate = __uint_as_float(odd ? away : raw[i]) * scale, up = __uint_as_float(odd ? raw[i + 1] : away) * scale;
+        *reinterpret_cast<T*>(staging + at * kStagingRow + lane / 2u * 2u) = from_float<T>(silu_f32(gate) * up);
+      }
+    } else {
+      const float bias = p.bias && column0 + lane < p.n ? as_float(reinterpret_cast<const T*>(p.bias)[column0 + lane]) : 0.0f;
+#pragma unroll
+      for (uint32_t i = 0; i < 32; ++i)
+        *reinterpret_cast<T*>(staging + i * kStagingRow + lane * 2u) = from_float<T>(__uint_as_float(raw[i]) + bias);
+    }
+    __syncwarp();
+    constexpr uint32_t kVectors = kPair ? 2 : 4;  // of a row
+    const uint32_t columns = kPair ? p.n / 2u : p.n, first = (kPair ? column0 / 2u : column0) + lane % kVectors * 8u;
+    const bool vectors = columns % 8u == 0 && ((uintptr_t)p.out & 15u) == 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kVectors; ++i) {
+      const uint32_t at = i * (32u / kVectors) + lane / kVectors;
+      if (row + at >= end || first >= columns) continue;
+      const uint4 eight = *reinterpret_cast<const uint4*>(staging + at * kStagingRow + lane % kVectors * 16u);
+      T* const out = reinterpret_cast<T*>(p.out) + (size_t)(row + at) * columns + first;
+      if (vectors) {
+        *reinterpret_cast<uint4*>(out) = eight;
+      } else {
+        const T* const values = reinterpret_cast<const T*>(&eight);
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j)
+          if (first + j < columns) out[j] = values[j];
+      }
+    }
+    __syncwarp();  // read before the next piece
+  }
+}
+
+template <Store S>
+__global__ void __launch_bounds__(kThreads, 1)
+tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Problem p, const Work work,
+             uint32_t* error_word) {
   extern __shared__ unsigned char shared_raw[];
   grid_chain_prologue();
   const uint32_t base = (smem_u32(shared_raw) + 1023u) & ~1023u;
   unsigned char* base_pointer = shared_raw + (base - smem_u32(shared_raw));
-  const uint32_t full = base + Z::kBarriers, scales_full = full + Z::kStages * 8, empty = scales_full + Z::kStages * 8;
-  const uint32_t sums_full = empty + Z::kStages * 8, sums_empty = sums_full + 16;
-  volatile uint32_t* holder = reinterpret_cast<volatile uint32_t*>(base_pointer + Z::kHolder);
-  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(base_pointer + Z::kAbort);
-  const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u;
+  const uint32_t full = base + kBarriers, scales_full = full + kStages * 8, empty = scales_full + kStages * 8;
+  const uint32_t sums_full = empty + kStages * 8, sums_empty = sums_full + kSums * 8, drained = sums_empty + kSums * 8;
+  volatile uint32_t* holder = reinterpret_cast<volatile uint32_t*>(base_pointer + kHolder);
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(base_pointer + kAbort);
+  const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u, rank = blockIdx.x & 1u, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const uint32_t row_tiles = p.plan.tiles ? min(p.plan.tiles[0], work.row_tiles) : work.row_tiles;
   const uint32_t tiles = row_tiles * work.column_tiles, k_stages = (p.k + kDepth - 1u) / kDepth;
-  auto place = [&](uint32_t tile) { return place_of<NT>(p, tile % row_tiles, 1u, tile / row_tiles * kColumns); };
+  auto place = [&](uint32_t tile) { return place_of(p, tile % row_tiles, work.rows, 1u, tile / row_tiles * 2u * kColumns); };
+  // rows that a product takes, half of them from either CTA: in boxes of 16 with a plan, otherwise in one of half the most rows
+  auto width = [&](const Place& at) { return max((at.end - at.row + 31u) / 32u * 32u, 32u); };
 
   if (threadIdx.x == 0) {
-    for (uint32_t s = 0; s < Z::kStages; ++s) {
-      barrier_init(full + s * 8, 1);  // the copies' expect_tx arrival; completes by byte count
-      barrier_init(scales_full + s * 8, kScaleWarps);
+    for (uint32_t s = 0; s < kStages; ++s) {
+      barrier_init(full + s * 8, 1);  // of the first CTA, for both: its expect_tx arrival; completes by byte count
+      barrier_init(scales_full + s * 8, 2 * kScaleWarps);  // the same
       barrier_init(empty + s * 8, 1);  // one tcgen05.commit
     }
-    for (uint32_t s = 0; s < 2; ++s) {
+    for (uint32_t s = 0; s < kSums; ++s) {
       barrier_init(sums_full + s * 8, 1);  // one tcgen05.commit
-      barrier_init(sums_empty + s * 8, Z::kEpilogueWarps);
+      barrier_init(sums_empty + s * 8, 2 * kEpilogueWarps);
     }
+    barrier_init(drained, 1);
     *abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + Z::kHolder), "r"(Z::kTmemColumns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + kHolder), "r"(kTmemColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  cluster_sync();  // either CTA's barriers are there for the other
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = uniform(*holder);
   auto give_up = [&]() {
@@ -83,13 +164,14 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   };
 
   if (warp == 0) {
-    uint32_t issued = 0, s = 0, phase = 1;  // stages over all tiles of this CTA
+    uint32_t issued = 0, s = 0, phase = 1;  // stages over all tiles of this pair
     bool ok = true;
-    for (uint32_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+    for (uint32_t tile = pair; tile < tiles && ok; tile += pairs) {
       const Place at = place(tile);
-      const uint32_t boxes = (at.end - at.row + work.box_rows - 1u) / work.box_rows;
+      const uint32_t half = uniform(width(at)) / 2u, x_row = uniform(at.row) + rank * half, w_row = uniform(at.w_row) + rank * kColumns;
+      const uint32_t boxes = p.plan.tiles ? half / work.box_rows : 1u;
       for (uint32_t ks = 0; ks < k_stages; ++ks, ++issued) {
-        const uint32_t stage = base + s * Z::kStageBytes;
+        const uint32_t stage = base + s * kStageBytes;
         ok = !*abort_flag && warp_wait(empty + s * 8, phase);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) {
@@ -97,178 +179,162 @@ product_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
           break;
         }
         if (elect_one()) {
-          barrier_expect_tx(full + s * 8, Z::kWeightBytes + boxes * work.box_rows * kRowBytes);
-          tma_load_2d(stage, &map_w, (int32_t)(ks * kRowBytes), (int32_t)at.w_row, full + s * 8);
+          const uint32_t first = first_address(full + s * 8);
+          if (rank == 0u) barrier_expect_tx(full + s * 8, 2u * (kWeightBytes + boxes * work.box_rows * kRowBytes));
+          pair_load(stage, &map_w, (int32_t)(ks * kRowBytes), (int32_t)w_row, first);
           for (uint32_t box = 0; box < boxes; ++box)
-            tma_load_2d(stage + Z::kWeightBytes + box * work.box_rows * kRowBytes, &map_x, (int32_t)(ks * kRowBytes),
-                        (int32_t)(at.row + box * work.box_rows), full + s * 8);
+            pair_load(stage + kWeightBytes + box * work.box_rows * kRowBytes, &map_x, (int32_t)(ks * kRowBytes), (int32_t)(x_row + box * work.box_rows), first);
         }
         __syncwarp();
-        if (++s == Z::kStages) s = 0, phase ^= 1u;
+        if (++s == kStages) s = 0, phase ^= 1u;
       }
     }
-    // on the way out after a failure the copies already started must land first
-    if (!ok || *abort_flag)
-      for (uint32_t i = issued > Z::kStages ? issued - Z::kStages : 0u; i < issued; ++i)
-        barrier_wait(full + (i % Z::kStages) * 8, (i / Z::kStages) & 1u);
+    // on the way out after a failure the copies already started must land first: both CTAs' have when the first one's barriers say so
+    if (rank == 0u && (!ok || *abort_flag))
+      for (uint32_t i = issued > kStages ? issued - kStages : 0u; i < issued; ++i) barrier_wait(full + (i % kStages) * 8, (i / kStages) & 1u);
     __syncwarp();
+  } else if (warp == 1 && rank == 1u) {
+    // the first CTA issues for both
   } else if (warp == 1) {
-    uint32_t s = 0, phase = 0, half = 0, turn = 0;
+    uint32_t s = 0, phase = 0, buffer = 0, turn = 0;
     bool ok = true;
-    for (uint32_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++turn) {
-      uint32_t rows = NT;
-      if (p.plan.tiles) {
-        const Place at = place(tile);
-        rows = uniform(max((at.end - at.row + 15u) / 16u * 16u, 16u));
-      }
-      const uint32_t low = mxf4_instruction(rows, 0u), high = mxf4_instruction(rows, 1u);
-      const uint32_t which = turn % Z::kSums, sums = tmem_base + which * NT;
-      ok = !*abort_flag && warp_wait(sums_empty + which * 8, ((turn / Z::kSums) & 1u) ^ 1u);
+    for (uint32_t tile = pair; tile < tiles && ok; tile += pairs, ++turn) {
+      const uint32_t rows = uniform(width(place(tile)));
+      const uint32_t low = mxf4_instruction(2u * kColumns, rows, 0u), high = mxf4_instruction(2u * kColumns, rows, 1u);
+      const uint32_t which = turn % kSums, sums = tmem_base + which * kMostRows;
+      ok = !*abort_flag && warp_wait(sums_empty + which * 8, ((turn / kSums) & 1u) ^ 1u);
       ok = __all_sync(0xffffffffu, ok);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       for (uint32_t ks = 0; ks < k_stages && ok; ++ks) {
-        const uint32_t stage = base + s * Z::kStageBytes;
+        const uint32_t stage = base + s * kStageBytes;
         ok = !*abort_flag && warp_wait(full + s * 8, phase) && warp_wait(scales_full + s * 8, phase);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t scales = tmem_base + Z::kSums * NT + half * Z::kScaleColumns, left = p.k - ks * kDepth;
-        const uint64_t a = operand_descriptor(stage), b = operand_descriptor(stage + Z::kWeightBytes);
+        const uint32_t scales = tmem_base + kSums * kMostRows + buffer * kScaleColumns, left = p.k - ks * kDepth;
+        const uint64_t a = operand_descriptor(stage), b = operand_descriptor(stage + kWeightBytes);
         if (elect_one()) {
 #pragma unroll
           for (uint32_t g = 0; g < kStageWords; ++g) {
             if (g * kWordValues >= left) break;
-            const uint32_t columns = scales + g * 4u * (1u + Z::kAtoms), atoms = stage + Z::kScalesAt + g * (1u + Z::kAtoms) * kAtom;
-#pragma unroll
-            for (uint32_t atom = 0; atom <= Z::kAtoms; ++atom) copy_atom(columns + atom * 4u, atoms + atom * kAtom);
+            const uint32_t columns = scales + g * 4u * (1u + kInputAtoms), atoms = stage + kInputScalesAt + g * kInputAtoms * kAtom;
+            pair_copy_atom(columns, stage + kScalesAt + g * kAtom);
+            pair_copy_atom(columns + 4u, atoms);
+            if (rows > 128u) pair_copy_atom(columns + 8u, atoms + kAtom);
           }
 #pragma unroll
           for (uint32_t j = 0; j < kDepth / 64; ++j) {
             if (j * 64u >= left) break;
-            const uint32_t columns = scales + j / 2u * 4u * (1u + Z::kAtoms);
-            mma_mxf4(sums, a + j * 2u, b + j * 2u, j & 1u ? high : low, columns, columns + 4u, (ks > 0 || j > 0) ? 1u : 0u);
+            const uint32_t columns = scales + j / 2u * 4u * (1u + kInputAtoms);
+            pair_mma(sums, a + j * 2u, b + j * 2u, j & 1u ? high : low, columns, columns + 4u, (ks > 0 || j > 0) ? 1u : 0u);
           }
-          mma_commit(empty + s * 8);
-          if (ks + 1u == k_stages) mma_commit(sums_full + which * 8);
+          pair_commit(empty + s * 8);
+          if (ks + 1u == k_stages) pair_commit(sums_full + which * 8);
         }
         __syncwarp();
-        half ^= 1u;
-        if (++s == Z::kStages) s = 0, phase ^= 1u;
+        buffer ^= 1u;
+        if (++s == kStages) s = 0, phase ^= 1u;
       }
     }
-    if (!ok) give_up();
+    if (!ok) {
+      // the products already issued read both CTAs' memory
+      give_up();
+      if (elect_one())
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drained) : "memory");
+      __syncwarp();
+      warp_wait(drained, 0u);
+    }
   } else if (warp < 2u + kScaleWarps) {
-    // a thread per row: its words of a stage, of the weights and of x
-    constexpr uint32_t kWords = kStageWords * (1 + Z::kAtoms);
-    const uint32_t t = (warp - 2u) * 32u + lane, words = words_of(p.k), target = (t & 31u) * 16u + (t >> 5) * 4u, last_mask = last_word_mask(p.k);
-      uint32_t held[kAhead][kWords];
-    uint32_t ahead_tile = blockIdx.x, ahead_stage = 0, mine = 0, left_tiles = 0;
-    for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) ++left_tiles;
-    const uint32_t all = left_tiles * k_stages;
+    // the words of a group of a stage: of the CTA's weight rows, or of the tile's rows of x, lane, lane + 32, ...
+    const uint32_t group = (warp - 2u) % kStageWords, words = words_of(p.k), last_mask = last_word_mask(p.k);
+    const bool of_x = warp - 2u >= kStageWords;
+    constexpr uint32_t kWords = kMostRows / 32;
+    uint32_t held[kAhead][kWords];
+    uint32_t all = 0, mine = 0, ahead_tile = pair, ahead_stage = 0;
+    for (uint32_t tile = pair; tile < tiles; tile += pairs) all += k_stages;
     Place ahead = {};
-    if (all > 0) ahead = place(blockIdx.x);
+    if (all > 0) ahead = place(pair);
+    // Nothing looks at them before they are laid down, so that nothing waits for them here.
     auto fetch = [&](uint32_t (&into)[kWords]) {
       if (mine >= all) return;
       ++mine;
+      const uint32_t at = ahead_stage * kStageWords + group;
+      const uint32_t* const source = of_x ? p.x_scales + (size_t)at * p.m : p.w_scales + (size_t)at * p.w_rows;
+      const uint32_t first = of_x ? ahead.row : ahead.w_row + rank * kColumns, end = at >= words ? 0u : of_x ? ahead.end : min(p.w_rows, first + kColumns);
 #pragma unroll
-      for (uint32_t g = 0; g < kStageWords; ++g) {
-        const uint32_t group = ahead_stage * kStageWords + g, w_row = ahead.w_row + t;
-        uint32_t& of_w = into[g * (1 + Z::kAtoms)];
-        of_w = 0u;
-        if (group < words && w_row < p.w_rows) of_w = p.w_scales[(size_t)group * p.w_rows + w_row];
-#pragma unroll
-        for (uint32_t a = 0; a < Z::kAtoms; ++a) {
-          const uint32_t row = ahead.row + a * 128u + t;
-          uint32_t& of_x = into[g * (1 + Z::kAtoms) + 1 + a];
-          of_x = 0u;
-          if (group < words && row < ahead.end) of_x = p.x_scales[(size_t)group * p.m + row];
-        }
+      for (uint32_t i = 0; i < kWords; ++i) {
+        into[i] = 0u;
+        if (first + i * 32u + lane < end) into[i] = source[first + i * 32u + lane];
       }
       if (++ahead_stage == k_stages) {
         ahead_stage = 0;
-        ahead_tile += gridDim.x;
+        ahead_tile += pairs;
         if (mine < all) ahead = place(ahead_tile);
       }
     };
 #pragma unroll
     for (uint32_t a = 0; a < kAhead; ++a) fetch(held[a]);
+    uint32_t s = 0, phase = 1, ks = 0;
     bool ok = true;
     for (uint32_t first = 0; first < all && ok; first += kAhead) {
 #pragma unroll
       for (uint32_t a = 0; a < kAhead; ++a) {
-        const uint32_t i = first + a, s = i % Z::kStages;
-        if (i >= all || !ok) break;
-        ok = !*abort_flag && barrier_wait(empty + s * 8, ((i / Z::kStages) & 1u) ^ 1u);
+        if (first + a >= all || !ok) break;
+        ok = !*abort_flag && warp_wait(empty + s * 8, phase);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        unsigned char* atoms = base_pointer + s * Z::kStageBytes + Z::kScalesAt + target;
-#pragma unroll
-        for (uint32_t w = 0; w < kWords; ++w)
-          *reinterpret_cast<uint32_t*>(atoms + w * kAtom) =
-              held[a][w] & (i % k_stages * kStageWords + w / (1 + Z::kAtoms) + 1u == words ? last_mask : 0xffffffffu);
+        const uint32_t mask = ks * kStageWords + group + 1u == words ? last_mask : 0xffffffffu;
+        const uint32_t(&v)[kWords] = held[a];
+        unsigned char* const line = base_pointer + s * kStageBytes + (of_x ? kInputScalesAt + group * kInputAtoms * kAtom : kScalesAt + group * kAtom) + lane * 16u;
+        *reinterpret_cast<uint4*>(line) = make_uint4(v[0] & mask, v[1] & mask, v[2] & mask, v[3] & mask);
+        if (of_x) *reinterpret_cast<uint4*>(line + kAtom) = make_uint4(v[4] & mask, v[5] & mask, v[6] & mask, 0u);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) barrier_arrive(scales_full + s * 8);
+        if (lane == 0) first_arrive(first_address(scales_full + s * 8));
         fetch(held[a]);
+        if (++ks == k_stages) ks = 0;
+        if (++s == kStages) s = 0, phase ^= 1u;
       }
     }
     if (!ok) give_up();
   } else {
-    const uint32_t worker = warp - 2u - kScaleWarps, quarter = warp & 3u, side = worker >> 2;  // lanes of tensor memory; share of the columns
-    constexpr uint32_t kPiece = 32, kSides = Z::kEpilogueWarps / 4;
+    const uint32_t worker = warp - 2u - kScaleWarps, quarter = warp & 3u, side = worker >> 2;  // lanes of tensor memory; every other piece
+    unsigned char* const staging = base_pointer + kStaging + worker * kStagingBytes;
     uint32_t turn = 0;
     bool ok = true;
-    for (uint32_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++turn) {
-      const uint32_t which = turn % Z::kSums;
+    for (uint32_t tile = pair; tile < tiles && ok; tile += pairs, ++turn) {
+      const uint32_t which = turn % kSums;
       const Place at = place(tile);
-      ok = !*abort_flag && barrier_wait(sums_full + which * 8, (turn / Z::kSums) & 1u);
+      ok = !*abort_flag && warp_wait(sums_full + which * 8, (turn / kSums) & 1u);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
         give_up();
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t address = tmem_base + which * NT + ((quarter * 32u) << 16);
+      const uint32_t address = tmem_base + which * kMostRows + ((quarter * 32u) << 16), column = at.column + rank * kColumns + quarter * 32u;
 #pragma unroll 1
-      for (uint32_t piece = side; piece < NT / kPiece; piece += kSides) {
-        const uint32_t row = at.row + piece * kPiece;
+      for (uint32_t piece = side; piece < kMostRows / 32u; piece += kEpilogueWarps / 4u) {
+        const uint32_t row = at.row + piece * 32u;
         if (row >= at.end) break;
-        uint32_t raw[kPiece];
-        tmem_load_32(address + piece * kPiece, raw);
+        uint32_t raw[32];
+        tmem_load_32(address + piece * 32u, raw);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        store_rows<S>(p, row, at.end, at.column + quarter * 32u + lane, raw);
+        store_piece<S>(p, row, at.end, column, raw, staging);
         __syncwarp();  // tcgen05.ld needs the whole warp
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) barrier_arrive(sums_empty + which * 8);
+      if (lane == 0) first_arrive(first_address(sums_empty + which * 8));
     }
   }
 
   __syncthreads();
+  cluster_sync();  // neither CTA leaves, or gives its tensor memory back, while the other's products or arrivals reach it
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(Z::kTmemColumns) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemColumns) : "memory");
   }
-}
-
-template <uint32_t NT, Store S>
-int run(const KernelArgs& args, const Problem& p, uint32_t row_tiles) {
-  using Z = Shape<NT>;
-  const uint32_t sms = (uint32_t)context_sm_count(args.ctx);
-  const Work work = {row_tiles, (p.n + kColumns - 1u) / kColumns, p.plan.tiles ? 32u : NT};
-  const size_t tiles = (size_t)work.row_tiles * work.column_tiles;
-  LLMOPT_REQUIRE(tiles < (1u << 28), "too many tiles");
-  CUtensorMap map_w, map_x;
-  LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.box_rows), "tensor map was refused");
-  auto kernel = product_kernel<NT, S>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::kSharedBytes) != cudaSuccess) {
-    cudaGetLastError();
-    return fail(args, "shared memory request was refused");
-  }
-  launch_kernel(args, kernel, dim3(tiles < sms ? (uint32_t)tiles : sms), dim3(Z::kThreads), Z::kSharedBytes, map_w, map_x, p, work,
-                context_device_error(args.ctx));
-  return check_launch(args);
 }
 
 }  // namespace
@@ -277,9 +343,26 @@ namespace mxfp4 {
 
 template <Store S>
 int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
-  auto tiles = [&](uint32_t rows) { return p.plan.tiles ? plan_tiles : (p.m + rows - 1u) / rows; };
-  if (p.m <= 128u || p.plan.tiles) return run<128, S>(args, p, tiles(128));
-  return run<256, S>(args, p, tiles(256));
+  const uint32_t pairs = (uint32_t)context_sm_count(args.ctx) / 2u, k_stages = (p.k + kDepth - 1u) / kDepth;
+  Work work = {plan_tiles, (p.n + 2u * kColumns - 1u) / (2u * kColumns), kExpertTile, 16u};
+  if (!p.plan.tiles) {
+    // the height with the shortest estimate: rounds of tiles times the cycles of one, of which a stage takes about 280 and one per row
+    uint64_t least = ~0ull;
+    for (uint32_t rows = kMostRows; rows >= 32u; rows -= 32u) {
+      const uint32_t row_tiles = (p.m + rows - 1u) / rows;
+      const uint64_t rounds = ((uint64_t)row_tiles * work.column_tiles + pairs - 1u) / pairs, cost = rounds * ((uint64_t)k_stages * (280u + rows) + 1000u);
+      if (cost < least) least = cost, work.rows = rows, work.row_tiles = row_tiles;
+    }
+    work.box_rows = work.rows / 2u;
+  }
+  const uint64_t tiles = (uint64_t)work.row_tiles * work.column_tiles;
+  LLMOPT_REQUIRE(tiles < (1u << 28), "too many tiles");
+  CUtensorMap map_w, map_x;
+  LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.box_rows), "tensor map was refused");
+  LLMOPT_REQUIRE((allow_shared<kSharedBytes, tiles_kernel<S>>()), "shared memory request was refused");
+  launch_cluster_kernel(args, tiles_kernel<S>, dim3(2u * (tiles < pairs ? (uint32_t)tiles : pairs)), dim3(kThreads), kSharedBytes, 2u, map_w, map_x, p,
+                        work, context_device_error(args.ctx));
+  return check_launch(args);
 }
 
 template int run_tiles<kStoreHalf>(const KernelArgs&, const Problem&, uint32_t);
