@@ -68,6 +68,10 @@ template <> struct Element<kStorePairBf16> { typedef bf16 Type; };
 __device__ __forceinline__ uint32_t packed(__half a, __half b) { return (uint32_t)__half_as_ushort(a) | (uint32_t)__half_as_ushort(b) << 16; }
 __device__ __forceinline__ uint32_t packed(bf16 a, bf16 b) { return (uint32_t)__bfloat16_as_ushort(a) | (uint32_t)__bfloat16_as_ushort(b) << 16; }
 
+// silu whose exponential and quotient are off by two steps of fp32 each, and by one of the exponent: of a result in sixteen bits that is
+// nothing, and with the exact quotient the pairs of a tile took longer than its products (9.0 against 5.2 us).
+__device__ __forceinline__ float silu_short(float z) { return __fdividef(z, 1.0f + __expf(-z)); }
+
 // Sums of COUNT rows from `row` on, of the output column that is this lane's, on their way out; the whole warp takes part.  Sixteen-bit
 // results go two columns at a time: neighbouring lanes exchange the sums of every other row.
 template <Store S, int COUNT>
@@ -98,7 +102,7 @@ __device__ __forceinline__ void store_rows(const Problem& p, uint32_t row, uint3
       if (at >= end || even_column >= p.n) continue;
       if constexpr (kPair) {
         const float scale = p.row_scale[at];
-        reinterpret_cast<T*>(p.out)[(size_t)at * (p.n / 2u) + even_column / 2u] = from_float<T>(silu_f32(first * scale) * (second * scale));
+        reinterpret_cast<T*>(p.out)[(size_t)at * (p.n / 2u) + even_column / 2u] = from_float<T>(silu_short(first * scale) * (second * scale));
       } else {
         T* out = reinterpret_cast<T*>(p.out) + (size_t)at * p.n + even_column;
         const T low = from_float<T>(first + bias[0]), high = from_float<T>(second + bias[1]);

@@ -1,4 +1,4 @@
-// Products of many MXFP4 rows: pairs of CTAs walk over tiles of 256 weight rows by up to 224 rows of x.
+// Products of many MXFP4 rows: pairs of CTAs walk over tiles of 256 weight rows by up to 224 rows of x (256 where no pair has a second tile).
 //
 // What bounds a tile is how often its operands come from L2: tcgen05.mma with cta_group::2 multiplies 256 weight rows, half of them in
 // either CTA's shared memory, with rows of x of which either CTA holds half as well, 30 KB for what a CTA by itself needs 44 KB for.
@@ -18,12 +18,12 @@ namespace {
 using namespace mxfp4;
 
 constexpr uint32_t kAhead = 4, kDepth = kBoxDepth, kStageWords = kDepth / kWordValues;  // of a stage
-constexpr uint32_t kMostRows = 224, kInputAtoms = 2;
+constexpr uint32_t kMostRows = 224, kLoneRows = 256, kInputAtoms = 2;  // of a tile; of the only one of every pair
 constexpr uint32_t kEpilogueWarps = 8, kThreads = (2 + kScaleWarps + kEpilogueWarps) * 32;
-constexpr uint32_t kWeightBytes = kColumns * kRowBytes, kInputBytes = kMostRows / 2 * kRowBytes;
+constexpr uint32_t kWeightBytes = kColumns * kRowBytes, kInputBytes = kLoneRows / 2 * kRowBytes;
 constexpr uint32_t kScalesAt = kWeightBytes + kInputBytes, kInputScalesAt = kScalesAt + kStageWords * kAtom;
 constexpr uint32_t kStageBytes = kInputScalesAt + kStageWords * kInputAtoms * kAtom;
-constexpr uint32_t kStages = 6, kSums = 2;
+constexpr uint32_t kStages = 5, kSums = 2;
 constexpr uint32_t kScaleColumns = kStageWords * 4 * (1 + kInputAtoms), kTmemColumns = 512;
 static_assert(kSums * kMostRows + 2 * kScaleColumns <= kTmemColumns && kStageBytes % 1024 == 0, "tensor memory, alignment of tiles");
 constexpr uint32_t kStagingRow = 80, kStagingBytes = 32 * kStagingRow;  // a warp's 32 rows of 64 bytes and 16 of padding
@@ -80,12 +80,13 @@ __device__ __forceinline__ void store_piece(const Problem& p, uint32_t row, uint
   } else {
     if constexpr (kPair) {
       const bool odd = lane & 1u;
+      const float scales = row + lane < end ? p.row_scale[row + lane] : 0.0f;
 #pragma unroll
       for (uint32_t i = 0; i < 32; i += 2) {
         const uint32_t away = __shfl_xor_sync(0xffffffffu, odd ? raw[i] : raw[i + 1], 1), at = i + (odd ? 1u : 0u);
-        const float scale = row + at < end ? p.row_scale[row + at] : 0.0f;
+        const float scale = __shfl_sync(0xffffffffu, scales, at);
         const float gate = __uint_as_float(odd ? away : raw[i]) * scale, up = __uint_as_float(odd ? raw[i + 1] : away) * scale;
-        *reinterpret_cast<T*>(staging + at * kStagingRow + lane / 2u * 2u) = from_float<T>(silu_f32(gate) * up);
+        *reinterpret_cast<T*>(staging + at * kStagingRow + lane / 2u * 2u) = from_float<T>(silu_short(gate) * up);
       }
     } else {
       const float bias = p.bias && column0 + lane < p.n ? as_float(reinterpret_cast<const T*>(p.bias)[column0 + lane]) : 0.0f;
@@ -248,7 +249,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     // the words of a group of a stage: of the CTA's weight rows, or of the tile's rows of x, lane, lane + 32, ...
     const uint32_t group = (warp - 2u) % kStageWords, words = words_of(p.k), last_mask = last_word_mask(p.k);
     const bool of_x = warp - 2u >= kStageWords;
-    constexpr uint32_t kWords = kMostRows / 32;
+    constexpr uint32_t kWords = kLoneRows / 32;
     uint32_t held[kAhead][kWords];
     uint32_t all = 0, mine = 0, ahead_tile = pair, ahead_stage = 0;
     for (uint32_t tile = pair; tile < tiles; tile += pairs) all += k_stages;
@@ -287,7 +288,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         const uint32_t(&v)[kWords] = held[a];
         unsigned char* const line = base_pointer + s * kStageBytes + (of_x ? kInputScalesAt + group * kInputAtoms * kAtom : kScalesAt + group * kAtom) + lane * 16u;
         *reinterpret_cast<uint4*>(line) = make_uint4(v[0] & mask, v[1] & mask, v[2] & mask, v[3] & mask);
-        if (of_x) *reinterpret_cast<uint4*>(line + kAtom) = make_uint4(v[4] & mask, v[5] & mask, v[6] & mask, 0u);
+        if (of_x) *reinterpret_cast<uint4*>(line + kAtom) = make_uint4(v[4] & mask, v[5] & mask, v[6] & mask, v[7] & mask);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) first_arrive(first_address(scales_full + s * 8));
@@ -314,7 +315,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t address = tmem_base + which * kMostRows + ((quarter * 32u) << 16), column = at.column + rank * kColumns + quarter * 32u;
 #pragma unroll 1
-      for (uint32_t piece = side; piece < kMostRows / 32u; piece += kEpilogueWarps / 4u) {
+      for (uint32_t piece = side; piece < kLoneRows / 32u; piece += kEpilogueWarps / 4u) {
         const uint32_t row = at.row + piece * 32u;
         if (row >= at.end) break;
         uint32_t raw[32];
@@ -348,8 +349,9 @@ int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
   if (!p.plan.tiles) {
     // the height with the shortest estimate: rounds of tiles times the cycles of one, of which a stage takes about 280 and one per row
     uint64_t least = ~0ull;
-    for (uint32_t rows = kMostRows; rows >= 32u; rows -= 32u) {
+    for (uint32_t rows = kLoneRows; rows >= 32u; rows -= 32u) {
       const uint32_t row_tiles = (p.m + rows - 1u) / rows;
+      if (rows > kMostRows && (uint64_t)row_tiles * work.column_tiles > pairs) continue;  // its sums lie over those of the next
       const uint64_t rounds = ((uint64_t)row_tiles * work.column_tiles + pairs - 1u) / pairs, cost = rounds * ((uint64_t)k_stages * (280u + rows) + 1000u);
       if (cost < least) least = cost, work.rows = rows, work.row_tiles = row_tiles;
     }
