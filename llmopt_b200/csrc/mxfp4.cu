@@ -13,90 +13,120 @@ namespace llmopt {
 namespace {
 using namespace mxfp4;
 
+// A CTA takes 32 rows x 256 columns, a warp four of the rows, 16 bytes of values per lane and access: 256 columns of 16 bits at a
+// time, 128 of 32.  The exponents of the 32 rows leave together, 128 bytes of a word's row.
 constexpr uint32_t kTileRows = 32, kTileColumns = 256, kWarps = 8, kRowsPerWarp = kTileRows / kWarps;
-
-// Eight values of a row as floats.
 template <typename T>
-__device__ __forceinline__ void load_eight(const T* source, bool vectors, float (&v)[8]) {
-  if (vectors) {
-    constexpr int kLoads = sizeof(T) / 2;
-    uint4 raw[kLoads];
+struct Access {
+  static constexpr uint32_t kValues = 16 / sizeof(T), kColumns = 32 * kValues, kPasses = kTileColumns / kColumns;
+  static constexpr uint32_t kBlockLanes = kBlock / kValues, kWordLanes = kWordValues / kValues;
+};
+
+template <typename T>
+__device__ __forceinline__ uint4 load_values(const T* source, bool vectors) {
+  if (vectors) return *reinterpret_cast<const uint4*>(source);
+  uint4 raw;
+  T* const values = reinterpret_cast<T*>(&raw);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) raw[i] = reinterpret_cast<const uint4*>(source)[i];
-    const T* values = reinterpret_cast<const T*>(raw);
+  for (uint32_t i = 0; i < Access<T>::kValues; ++i) values[i] = source[i];
+  return raw;
+}
+// The largest size among a lane's values, as the bits of a float: sizes compare as integers, NaN above infinity.  Sixteen-bit types
+// compare two at a time and by themselves.
+__device__ __forceinline__ uint32_t largest_pair(const uint4& raw) {
+  uint32_t most = raw.x & 0x7fff7fffu;
+  asm("max.u16x2 %0, %0, %1;" : "+r"(most) : "r"(raw.y & 0x7fff7fffu));
+  asm("max.u16x2 %0, %0, %1;" : "+r"(most) : "r"(raw.z & 0x7fff7fffu));
+  asm("max.u16x2 %0, %0, %1;" : "+r"(most) : "r"(raw.w & 0x7fff7fffu));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = as_float(values[i]);
-    return;
+  for (uint32_t offset = 1; offset < Access<__half>::kBlockLanes; offset <<= 1) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, most, offset);
+    asm("max.u16x2 %0, %0, %1;" : "+r"(most) : "r"(other));
   }
+  return max(most & 0xffffu, most >> 16);
+}
+__device__ __forceinline__ uint32_t largest(const uint4& raw, __half) {
+  return __float_as_uint(__half2float(__ushort_as_half((uint16_t)largest_pair(raw))));
+}
+__device__ __forceinline__ uint32_t largest(const uint4& raw, bf16) { return largest_pair(raw) << 16; }
+__device__ __forceinline__ uint32_t largest(const uint4& raw, float) {
+  uint32_t most = max(max(raw.x & 0x7fffffffu, raw.y & 0x7fffffffu), max(raw.z & 0x7fffffffu, raw.w & 0x7fffffffu));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = as_float(source[i]);
+  for (uint32_t offset = 1; offset < Access<float>::kBlockLanes; offset <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, offset));
+  return most;
+}
+// Codes of eight or four values times `inverse`.
+__device__ __forceinline__ uint32_t encode(const float (&v)[8], float inverse) {
+  uint32_t codes;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(codes)
+      : "f"(v[0] * inverse), "f"(v[1] * inverse), "f"(v[2] * inverse), "f"(v[3] * inverse), "f"(v[4] * inverse), "f"(v[5] * inverse),
+        "f"(v[6] * inverse), "f"(v[7] * inverse));
+  return codes;
+}
+__device__ __forceinline__ uint32_t encode(const float (&v)[4], float inverse) {
+  uint16_t codes;
+  asm("{\n\t.reg .b8 a, b;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\tmov.b16 %0, {a, b};\n\t}"
+      : "=h"(codes)
+      : "f"(v[0] * inverse), "f"(v[1] * inverse), "f"(v[2] * inverse), "f"(v[3] * inverse));
+  return codes;
+}
+// The codes of a lane's values: four bytes of eight, two of four.
+__device__ __forceinline__ void store_codes(uint8_t* target, uint32_t codes, __half) { *reinterpret_cast<uint32_t*>(target) = codes; }
+__device__ __forceinline__ void store_codes(uint8_t* target, uint32_t codes, bf16) { *reinterpret_cast<uint32_t*>(target) = codes; }
+__device__ __forceinline__ void store_codes(uint8_t* target, uint32_t codes, float) { *reinterpret_cast<uint16_t*>(target) = (uint16_t)codes; }
+template <typename T>
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* source) {
+  return sizeof(T) == 4 ? *reinterpret_cast<const uint16_t*>(source) : *reinterpret_cast<const uint32_t*>(source);
 }
 
-// A CTA takes 32 rows x 256 columns, a warp four of the rows, a lane eight neighbouring values.  Four lanes share a block, sixteen a
-// word of exponents; the words of the 32 rows leave together.
 template <typename T, bool GATHER>
-__global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const T* x, const uint32_t* index, uint8_t* codes, uint32_t* scales, uint32_t rows,
+__global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 4 ? 5 : 6) quantize_kernel(const T* x, const uint32_t* index, uint8_t* codes, uint32_t* scales, uint32_t rows,
                                                                uint32_t source_rows, uint32_t k, size_t stride, bool vectors) {
+  using A = Access<T>;
   grid_chain_prologue();
   __shared__ uint32_t words[2][kTileRows];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const uint32_t row0 = blockIdx.x * kTileRows, column = blockIdx.y * kTileColumns + lane * 8u;
-  float v[kRowsPerWarp][8];
+  const uint32_t row0 = blockIdx.x * kTileRows, column0 = blockIdx.y * kTileColumns + lane * A::kValues;
+  uint4 raw[kRowsPerWarp][A::kPasses];
+  uint32_t source[kRowsPerWarp];
 #pragma unroll
   for (uint32_t i = 0; i < kRowsPerWarp; ++i) {
     const uint32_t row = row0 + warp + i * kWarps;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-    if (row < rows && column < k) {
-      const uint32_t source = GATHER ? min(index[row], source_rows - 1u) : row;  // whatever the index says
-      load_eight(x + source * stride + column, vectors, v[i]);
-    }
+    source[i] = row < rows ? GATHER ? min(index[row], source_rows - 1u) : row : 0u;  // whatever the index says
   }
 #pragma unroll
-  for (uint32_t i = 0; i < kRowsPerWarp; ++i) {
-    const uint32_t at = warp + i * kWarps, row = row0 + at;
-    uint32_t most = 0;  // sizes compare as integers, NaN above infinity
+  for (uint32_t i = 0; i < kRowsPerWarp; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[i][j]) & 0x7fffffffu);
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const bool number = most < 0x7f800000u;
-    const uint32_t s = number ? max(most >> 23, 2u) - 2u : 255u;
-    const float inverse = __uint_as_float((254u - min(s, 253u)) << 23);
-    uint32_t packed = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t pair;
-      asm("{\n\t.reg .b8 b, z;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\n\tmov.b32 %0, {b, z, z, z};\n\t}"
-          : "=r"(pair)
-          : "f"(v[i][2 * j] * inverse), "f"(v[i][2 * j + 1] * inverse));
-      packed |= (pair & 255u) << (8 * j);
+    for (uint32_t pass = 0; pass < A::kPasses; ++pass) {
+      const uint32_t column = column0 + pass * A::kColumns;
+      raw[i][pass] = make_uint4(0u, 0u, 0u, 0u);
+      if (row0 + warp + i * kWarps < rows && column < k) raw[i][pass] = load_values(x + source[i] * stride + column, vectors);
     }
-    if (row < rows && column < k) *reinterpret_cast<uint32_t*>(codes + (size_t)row * (k / 2u) + column / 2u) = number ? packed : 0u;
-    uint32_t word = column < k ? s << (8u * (lane >> 2 & 3u)) : 0u;
-    word |= __shfl_xor_sync(0xffffffffu, word, 4);
-    word |= __shfl_xor_sync(0xffffffffu, word, 8);
-    if ((lane & 15u) == 0u) words[lane >> 4][at] = word;
-  }
+#pragma unroll
+  for (uint32_t i = 0; i < kRowsPerWarp; ++i)
+#pragma unroll
+    for (uint32_t pass = 0; pass < A::kPasses; ++pass) {
+      const uint32_t at = warp + i * kWarps, row = row0 + at, column = column0 + pass * A::kColumns;
+      const T* const values = reinterpret_cast<const T*>(&raw[i][pass]);
+      float v[A::kValues];
+#pragma unroll
+      for (uint32_t j = 0; j < A::kValues; ++j) v[j] = as_float(values[j]);
+      const uint32_t most = largest(raw[i][pass], T{});
+      const bool number = most < 0x7f800000u;
+      const uint32_t s = number ? max(most >> 23, 2u) - 2u : 255u;
+      const uint32_t packed = encode(v, __uint_as_float((254u - min(s, 253u)) << 23));
+      if (row < rows && column < k) store_codes(codes + (size_t)row * (k / 2u) + column / 2u, number ? packed : 0u, T{});
+      uint32_t word = column < k ? s << (8u * (lane / A::kBlockLanes & 3u)) : 0u;
+#pragma unroll
+      for (uint32_t offset = A::kBlockLanes; offset < A::kWordLanes; offset <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, offset);
+      if (lane % A::kWordLanes == 0u) words[pass * (A::kColumns / kWordValues) + lane / A::kWordLanes][at] = word;
+    }
   __syncthreads();
-  const uint32_t group = blockIdx.y * 2u + (threadIdx.x >> 5), row = row0 + lane;
-  if (threadIdx.x < 64u && group < words_of(k) && row < rows) scales[(size_t)group * rows + row] = words[threadIdx.x >> 5][lane];
-}
-
-template <typename T>
-__device__ __forceinline__ void store_eight(T* target, const float (&v)[8], bool vectors) {
-  constexpr int kStores = sizeof(T) / 2;
-  uint4 raw[kStores];
-  T* values = reinterpret_cast<T*>(raw);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) values[i] = from_float<T>(v[i]);
-  if (vectors) {
-#pragma unroll
-    for (int i = 0; i < kStores; ++i) reinterpret_cast<uint4*>(target)[i] = raw[i];
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) target[i] = values[i];
+  const uint32_t group = blockIdx.y * 2u + warp, row = row0 + lane;
+  if (warp < 2u && group < words_of(k) && row < rows) scales[(size_t)group * rows + row] = words[warp][lane];
 }
 
 // The same tiles the other way.  A value has two significant bits, so its product with the power of two is exact in fp32 and leaves
@@ -104,30 +134,44 @@ __device__ __forceinline__ void store_eight(T* target, const float (&v)[8], bool
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* codes, const uint32_t* scales, T* out, uint32_t rows, uint32_t k,
                                                                  bool vectors) {
+  using A = Access<T>;
   grid_chain_prologue();
   __shared__ uint32_t words[2][kTileRows];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const uint32_t row0 = blockIdx.x * kTileRows, column = blockIdx.y * kTileColumns + lane * 8u;
-  uint32_t packed[kRowsPerWarp];
+  const uint32_t row0 = blockIdx.x * kTileRows, column0 = blockIdx.y * kTileColumns + lane * A::kValues;
+  uint32_t packed[kRowsPerWarp][A::kPasses];
 #pragma unroll
-  for (uint32_t i = 0; i < kRowsPerWarp; ++i) {
-    const uint32_t row = row0 + warp + i * kWarps;
-    packed[i] = row < rows && column < k ? *reinterpret_cast<const uint32_t*>(codes + (size_t)row * (k / 2u) + column / 2u) : 0u;
-  }
+  for (uint32_t i = 0; i < kRowsPerWarp; ++i)
+#pragma unroll
+    for (uint32_t pass = 0; pass < A::kPasses; ++pass) {
+      const uint32_t row = row0 + warp + i * kWarps, column = column0 + pass * A::kColumns;
+      packed[i][pass] = row < rows && column < k ? load_codes<T>(codes + (size_t)row * (k / 2u) + column / 2u) : 0u;
+    }
   const uint32_t group = blockIdx.y * 2u + warp;
   if (warp < 2u) words[warp][lane] = group < words_of(k) && row0 + lane < rows ? scales[(size_t)group * rows + row0 + lane] : 0u;
   __syncthreads();
 #pragma unroll
-  for (uint32_t i = 0; i < kRowsPerWarp; ++i) {
-    const uint32_t at = warp + i * kWarps, row = row0 + at;
-    if (row >= rows || column >= k) continue;
-    const float scale = scale_value(words[lane >> 4][at] >> (8u * (lane >> 2 & 3u)) & 255u);
-    float v[8];
-    elements(packed[i], v);
+  for (uint32_t i = 0; i < kRowsPerWarp; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= scale;
-    store_eight(out + (size_t)row * k + column, v, vectors);
-  }
+    for (uint32_t pass = 0; pass < A::kPasses; ++pass) {
+      const uint32_t at = warp + i * kWarps, row = row0 + at, column = column0 + pass * A::kColumns;
+      if (row >= rows || column >= k) continue;
+      const uint32_t word = words[pass * (A::kColumns / kWordValues) + lane / A::kWordLanes][at];
+      const float scale = scale_value(word >> (8u * (lane / A::kBlockLanes & 3u)) & 255u);
+      float v[A::kValues];
+      elements(packed[i][pass], v);
+      uint4 raw;
+      T* const values = reinterpret_cast<T*>(&raw);
+#pragma unroll
+      for (uint32_t j = 0; j < A::kValues; ++j) values[j] = from_float<T>(v[j] * scale);
+      T* const target = out + (size_t)row * k + column;
+      if (vectors) {
+        *reinterpret_cast<uint4*>(target) = raw;
+      } else {
+#pragma unroll
+        for (uint32_t j = 0; j < A::kValues; ++j) target[j] = values[j];
+      }
+    }
 }
 
 bool aligned(const void* pointer) { return ((uintptr_t)pointer & 15u) == 0; }

@@ -27,10 +27,11 @@ __device__ __forceinline__ float scale_value(uint32_t s) {
   return __uint_as_float(s == 255u ? 0x7fffffffu : s == 0u ? 0x00400000u : s << 23);
 }
 
-// Eight elements of a word, the first in its lowest nibble.
-__device__ __forceinline__ void elements(uint32_t codes, float (&v)[8]) {
+// COUNT elements, the first in the lowest nibble; halves hold them exactly.
+template <uint32_t COUNT>
+__device__ __forceinline__ void elements(uint32_t codes, float (&v)[COUNT]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (uint32_t i = 0; i < COUNT / 2; ++i) {
     uint32_t pair;
     asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b0;\n\t}" : "=r"(pair) : "r"(codes >> (8 * i)));
     const float2 both = __half22float2(*reinterpret_cast<const __half2*>(&pair));
