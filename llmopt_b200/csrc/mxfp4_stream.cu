@@ -5,8 +5,6 @@
 // registers and laid down in the order that tcgen05.cp spreads over tensor memory; one lane of warp 1 issues copies and products; then
 // warps 2 to 5 read the sums out.  CTAs of a cluster hand each row's sums to the one that joins them, in the order of k.
 //
-// While the kernel before still runs, the tile's weights are asked into L2: that changes nothing that anybody reads, whoever writes them.
-//
 // Every wait on an mbarrier is bounded; a wait that runs out raises the context's device error word, and the CTA lets its copies land,
 // frees its tensor memory and returns.
 #include "mxfp4_tc.cuh"
@@ -37,7 +35,6 @@ struct Shape {
 struct Work {
   uint32_t row_tiles, column_tiles, splits, stages, box_rows;
   uint32_t share;  // rows that a CTA of a cluster joins
-  uint32_t parts;  // tiles here per tile of the plan, most often one of which has rows
 };
 // Shared memory, 1024 of it for the alignment of the ring; behind the barriers the sums of a cluster's CTAs, [from][row of the share][column],
 // and a row that may be read but not used.
@@ -71,7 +68,8 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
   volatile uint32_t* abort_flag = holder + 1;
   const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u;
   const uint32_t splits = work.splits, rank = blockIdx.x % splits, tile = blockIdx.x / splits;
-  const uint32_t column = tile / work.row_tiles * kColumns, k_stages = (p.k + kDepth - 1u) / kDepth;
+  // tiles that the plan does not have come last
+  const uint32_t row_tile = tile / work.column_tiles, column = tile % work.column_tiles * kColumns, k_stages = (p.k + kDepth - 1u) / kDepth;
   const uint32_t stage0 = k_stages * rank / splits, stage1 = k_stages * (rank + 1u) / splits, words = words_of(p.k);
 
   if (warp == 0) {
@@ -86,22 +84,12 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
-    if (!p.plan.tiles && elect_one())
-      for (uint32_t box = stage0 * kBoxes; box < stage1 * kBoxes && box * kBoxDepth < p.k; ++box)
-        asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(&map_w), "r"((int32_t)(box * kRowBytes)), "r"((int32_t)column)
-                     : "memory");
-    __syncwarp();
+    asm volatile("bar.arrive 1, %0;" ::"n"(kThreads) : "memory");
   }
-  if (warp >= 2 && !p.plan.tiles)
-    for (uint32_t group = stage0 * kStageWords + warp - 2u; group < min(stage1 * kStageWords, words); group += kStageWords)
-      if (const uint32_t row = column + lane * 32u; lane < kColumns / 32u && row < p.w_rows)
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(p.w_scales + (size_t)group * p.w_rows + row) : "memory");
   if (splits > 1u) cluster_arrive();  // this CTA runs: others may write into its shared memory
   grid_dependency_wait();
-  // whole clusters leave: those of tiles that the plan does not have, and of halves of its tiles without rows
-  if (p.plan.tiles && tile % work.row_tiles / work.parts >= min(p.plan.tiles[0], work.row_tiles / work.parts)) return;
-  const Place at = place_of(p, tile % work.row_tiles, NT, work.parts, column);
-  if (p.plan.tiles && at.row >= at.end) return;
+  if (p.plan.tiles && row_tile >= min(p.plan.tiles[0], work.row_tiles)) return;  // the whole cluster
+  const Place at = place_of(p, row_tile, NT, column);
 
   auto give_up = [&]() {
     *abort_flag = 1u;
@@ -149,10 +137,13 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 #pragma unroll
     for (uint32_t a = 0; a < kAhead; ++a) fetch(stage0 + a, held[a]);
   }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem_base = uniform(*holder);
+  // warp 0 has said that its barriers are there, and goes on to copy
+  if (warp > 0) {
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  }
+  const uint32_t tmem_base = warp > 0 ? uniform(*holder) : 0u;
 
   if (warp == 0) {
     bool ok = true;
@@ -253,7 +244,8 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         else tmem_load_32(address + piece * Z::kPiece, raw);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         if (splits == 1u) {
-          store_rows<S>(p, row, at.end, at.column + place, raw);
+          // through the ring: every stage of it has been read
+          store_piece<S>(p, row, at.end, at.column + quarter * 32u, raw, base_pointer + quarter * kStagingBytes);
         } else {
 #pragma unroll
           for (uint32_t i = 0; i < Z::kPiece; ++i) {
@@ -296,16 +288,15 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
 }
 
 template <uint32_t NT, Store S>
-int run(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
+int run(const KernelArgs& args, const Problem& p, uint32_t row_tiles) {
   using Z = Shape<NT>;
   const uint32_t sms = (uint32_t)context_sm_count(args.ctx), k_stages = (p.k + kDepth - 1u) / kDepth;
-  const uint32_t parts = p.m <= NT ? 1u : kExpertTile / NT;
-  Work work = {p.plan.tiles ? plan_tiles * parts : 1u, (p.n + kColumns - 1u) / kColumns, 1u, 0u, p.plan.tiles ? 16u : NT, 0u, parts};
+  Work work = {row_tiles, (p.n + kColumns - 1u) / kColumns, 1u, 0u, p.plan.tiles ? 16u : NT, 0u};
   const size_t tiles = (size_t)work.row_tiles * work.column_tiles;
   LLMOPT_REQUIRE(tiles < (1u << 28), "too many tiles");
   // CTAs that share a tile's k while tiles leave SMs without work; powers of two, which leave the fewest SMs of a GPC over.  us with 1, 2, 4, 8
   // of them: 4096 x 4096 6.3, 5.2, 4.3, 6.3; k 14336 x 4096 16.8, 11.5, 9.1, 18; 4096 x 14336 (112 tiles) 8.1, 12.
-  while (work.splits < kMostSplits && tiles * work.splits * 2u <= sms && k_stages >= work.splits * 2u) work.splits *= 2u;
+  while (work.splits < kMostSplits && tiles * work.splits * 2u <= sms && p.k / kDepth >= work.splits * 2u) work.splits *= 2u;
   const uint32_t mine = (k_stages + work.splits - 1u) / work.splits;
   // a CTA per SM: a deep ring; more: two of them per SM, which start and end beside one another (4 and 2 stages: 4096 x 14336 8.1, 10.1 us;
   // 4096 x 128256 57.9, 54.1)
@@ -313,6 +304,7 @@ int run(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
   work.stages = mine < most ? mine : most;
   const uint32_t rows = p.m < NT ? p.m : NT;
   work.share = (rows + work.splits - 1u) / work.splits;
+  while (shared_bytes<NT>(work) > kMostShared) --work.stages;
   CUtensorMap map_w, map_x;
   LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.box_rows), "tensor map was refused");
   auto kernel = stream_kernel<NT, S>;
@@ -332,9 +324,10 @@ namespace mxfp4 {
 
 template <Store S>
 int run_stream(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
-  if (p.m <= 16u) return run<16, S>(args, p, plan_tiles);
-  if (p.m <= 32u) return run<32, S>(args, p, plan_tiles);
-  return run<64, S>(args, p, plan_tiles);
+  const uint32_t row_tiles = p.plan.tiles ? plan_tiles : 1u;
+  if (p.m <= 16u) return run<16, S>(args, p, row_tiles);
+  if (p.m <= 32u) return run<32, S>(args, p, row_tiles);
+  return run<64, S>(args, p, row_tiles);
 }
 
 template int run_stream<kStoreHalf>(const KernelArgs&, const Problem&, uint32_t);

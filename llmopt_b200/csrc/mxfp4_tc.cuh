@@ -83,8 +83,10 @@ __device__ __forceinline__ void store_rows(const Problem& p, uint32_t row, uint3
     const float bias = p.bias ? reinterpret_cast<const float*>(p.bias)[column] : 0.0f;
     float* out = reinterpret_cast<float*>(p.out) + (size_t)row * p.n + column;
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i, out += p.n)
-      if (row + i < end) *out = __uint_as_float(raw[i]) + bias;
+    for (int i = 0; i < COUNT; ++i, out += p.n) {
+      if (row + i >= end) break;  // the same for the whole warp
+      *out = __uint_as_float(raw[i]) + bias;
+    }
   } else {
     const uint32_t even_column = column & ~1u;
     constexpr bool kPair = S == kStorePairHalf || S == kStorePairBf16;
@@ -96,6 +98,7 @@ __device__ __forceinline__ void store_rows(const Problem& p, uint32_t row, uint3
     const bool words = p.n % 2u == 0 && ((uintptr_t)p.out & 3u) == 0;
 #pragma unroll
     for (int i = 0; i < COUNT; i += 2) {
+      if (row + i >= end) break;  // the same for the whole warp
       const uint32_t away = __shfl_xor_sync(0xffffffffu, odd ? raw[i] : raw[i + 1], 1);
       const float first = __uint_as_float(odd ? away : raw[i]), second = __uint_as_float(odd ? raw[i + 1] : away);
       const uint32_t at = row + i + (odd ? 1 : 0);
@@ -117,17 +120,69 @@ __device__ __forceinline__ void store_rows(const Problem& p, uint32_t row, uint3
   }
 }
 
+constexpr uint32_t kStagingRow = 80, kStagingBytes = 32 * kStagingRow;  // a warp's 32 rows of 64 bytes and 16 of padding
+
+// The same of 16 or 32 rows from `row` on and the warp's 32 columns, through the warp's staging: lanes share the 64 bytes of a row.
+template <Store S, uint32_t COUNT>
+__device__ __forceinline__ void store_piece(const Problem& p, uint32_t row, uint32_t end, uint32_t column0, const uint32_t (&raw)[COUNT], unsigned char* staging) {
+  typedef typename Element<S>::Type T;
+  constexpr bool kPair = S == kStorePairHalf || S == kStorePairBf16;
+  const uint32_t lane = threadIdx.x & 31u;
+  if constexpr (S == kStoreFloat) {
+    store_rows<S>(p, row, end, column0 + lane, raw);
+  } else {
+    if constexpr (kPair) {
+      const bool odd = lane & 1u;
+      const float scales = row + lane < end ? p.row_scale[row + lane] : 0.0f;
+#pragma unroll
+      for (uint32_t i = 0; i < COUNT; i += 2) {
+        if (row + i >= end) break;  // the same for the whole warp
+        const uint32_t away = __shfl_xor_sync(0xffffffffu, odd ? raw[i] : raw[i + 1], 1), at = i + (odd ? 1u : 0u);
+        const float scale = __shfl_sync(0xffffffffu, scales, at);
+        const float gate = __uint_as_float(odd ? away : raw[i]) * scale, up = __uint_as_float(odd ? raw[i + 1] : away) * scale;
+        *reinterpret_cast<T*>(staging + at * kStagingRow + lane / 2u * 2u) = from_float<T>(silu_short(gate) * up);
+      }
+    } else {
+      const float bias = p.bias && column0 + lane < p.n ? as_float(reinterpret_cast<const T*>(p.bias)[column0 + lane]) : 0.0f;
+#pragma unroll
+      for (uint32_t i = 0; i < COUNT; ++i) {
+        if (row + i >= end) break;
+        *reinterpret_cast<T*>(staging + i * kStagingRow + lane * 2u) = from_float<T>(__uint_as_float(raw[i]) + bias);
+      }
+    }
+    __syncwarp();
+    constexpr uint32_t kVectors = kPair ? 2 : 4;  // of a row
+    const uint32_t columns = kPair ? p.n / 2u : p.n, first = (kPair ? column0 / 2u : column0) + lane % kVectors * 8u;
+    const bool vectors = columns % 8u == 0 && ((uintptr_t)p.out & 15u) == 0;
+#pragma unroll
+    for (uint32_t i = 0; i < COUNT * kVectors / 32; ++i) {
+      const uint32_t at = i * (32u / kVectors) + lane / kVectors;
+      if (row + at >= end || first >= columns) continue;
+      const uint4 eight = *reinterpret_cast<const uint4*>(staging + at * kStagingRow + lane % kVectors * 16u);
+      T* const out = reinterpret_cast<T*>(p.out) + (size_t)(row + at) * columns + first;
+      if (vectors) {
+        *reinterpret_cast<uint4*>(out) = eight;
+      } else {
+        const T* const values = reinterpret_cast<const T*>(&eight);
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j)
+          if (first + j < columns) out[j] = values[j];
+      }
+    }
+    __syncwarp();  // read before the next piece
+  }
+}
+
 // Rows of x that a tile multiplies, its first weight row, and the output column of that row.
 struct Place {
   uint32_t row, end, w_row, column;
 };
-// Tiles have at most `rows` rows; one of the plan is `parts` of them.
-__device__ __forceinline__ Place place_of(const Problem& p, uint32_t row_tile, uint32_t rows, uint32_t parts, uint32_t column) {
+// Tiles have at most `rows` rows; the plan's have no more of them than that.
+__device__ __forceinline__ Place place_of(const Problem& p, uint32_t row_tile, uint32_t rows, uint32_t column) {
   if (!p.plan.tiles) return {row_tile * rows, min(p.m, (row_tile + 1u) * rows), column, column};
-  const DenseTile tile = dense_tile(p.plan, row_tile / parts);
-  const uint32_t first = min(tile.first, p.m), last = max(first, min(min(tile.end, p.m), first + kExpertTile));  // whatever the plan says
-  const uint32_t row = min(first + row_tile % parts * rows, last);
-  return {row, min(last, row + rows), min(tile.expert, p.plan.experts - 1u) * p.n + column, column};
+  const DenseTile tile = dense_tile(p.plan, row_tile);  // whatever the plan says: rows that are there, and no more than a tile's
+  const uint32_t row = min(tile.first, p.m), end = max(row, min(min(tile.end, p.m), row + rows));
+  return {row, end, min(tile.expert, p.plan.experts - 1u) * p.n + column, column};
 }
 // Bytes of the last word that lie behind k hold no exponents.
 __device__ __forceinline__ uint32_t last_word_mask(uint32_t k) {

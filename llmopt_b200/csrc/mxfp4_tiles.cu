@@ -26,7 +26,6 @@ constexpr uint32_t kStageBytes = kInputScalesAt + kStageWords * kInputAtoms * kA
 constexpr uint32_t kStages = 5, kSums = 2;
 constexpr uint32_t kScaleColumns = kStageWords * 4 * (1 + kInputAtoms), kTmemColumns = 512;
 static_assert(kSums * kMostRows + 2 * kScaleColumns <= kTmemColumns && kStageBytes % 1024 == 0, "tensor memory, alignment of tiles");
-constexpr uint32_t kStagingRow = 80, kStagingBytes = 32 * kStagingRow;  // a warp's 32 rows of 64 bytes and 16 of padding
 constexpr uint32_t kStaging = kStages * kStageBytes, kBarriers = kStaging + kEpilogueWarps * kStagingBytes;
 constexpr uint32_t kHolder = kBarriers + (3 * kStages + 2 * kSums + 1) * 8, kAbort = kHolder + 4;
 constexpr uint32_t kSharedBytes = kAbort + 4 + 1024;  // slack: 1024-byte alignment of the tiles
@@ -69,54 +68,6 @@ __device__ __forceinline__ void pair_commit(uint32_t bar) {
                : "memory");
 }
 
-// 32 rows of sums of this lane's column, on their way out through the warp's staging.
-template <Store S>
-__device__ __forceinline__ void store_piece(const Problem& p, uint32_t row, uint32_t end, uint32_t column0, const uint32_t (&raw)[32], unsigned char* staging) {
-  typedef typename Element<S>::Type T;
-  constexpr bool kPair = S == kStorePairHalf || S == kStorePairBf16;
-  const uint32_t lane = threadIdx.x & 31u;
-  if constexpr (S == kStoreFloat) {
-    store_rows<S>(p, row, end, column0 + lane, raw);
-  } else {
-    if constexpr (kPair) {
-      const bool odd = lane & 1u;
-      const float scales = row + lane < end ? p.row_scale[row + lane] : 0.0f;
-#pragma unroll
-      for (uint32_t i = 0; i < 32; i += 2) {
-        const uint32_t away = __shfl_xor_sync(0xffffffffu, odd ? raw[i] : raw[i + 1], 1), at = i + (odd ? 1u : 0u);
-        const float scale = __shfl_sync(0xffffffffu, scales, at);
-        const float gate = __uint_as_float(odd ? away : raw[i]) * scale, up = __uint_as_float(odd ? raw[i + 1] : away) * scale;
-        *reinterpret_cast<T*>(staging + at * kStagingRow + lane / 2u * 2u) = from_float<T>(silu_short(gate) * up);
-      }
-    } else {
-      const float bias = p.bias && column0 + lane < p.n ? as_float(reinterpret_cast<const T*>(p.bias)[column0 + lane]) : 0.0f;
-#pragma unroll
-      for (uint32_t i = 0; i < 32; ++i)
-        *reinterpret_cast<T*>(staging + i * kStagingRow + lane * 2u) = from_float<T>(__uint_as_float(raw[i]) + bias);
-    }
-    __syncwarp();
-    constexpr uint32_t kVectors = kPair ? 2 : 4;  // of a row
-    const uint32_t columns = kPair ? p.n / 2u : p.n, first = (kPair ? column0 / 2u : column0) + lane % kVectors * 8u;
-    const bool vectors = columns % 8u == 0 && ((uintptr_t)p.out & 15u) == 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kVectors; ++i) {
-      const uint32_t at = i * (32u / kVectors) + lane / kVectors;
-      if (row + at >= end || first >= columns) continue;
-      const uint4 eight = *reinterpret_cast<const uint4*>(staging + at * kStagingRow + lane % kVectors * 16u);
-      T* const out = reinterpret_cast<T*>(p.out) + (size_t)(row + at) * columns + first;
-      if (vectors) {
-        *reinterpret_cast<uint4*>(out) = eight;
-      } else {
-        const T* const values = reinterpret_cast<const T*>(&eight);
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j)
-          if (first + j < columns) out[j] = values[j];
-      }
-    }
-    __syncwarp();  // read before the next piece
-  }
-}
-
 template <Store S>
 __global__ void __launch_bounds__(kThreads, 1)
 tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Problem p, const Work work,
@@ -132,7 +83,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
   const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u, rank = blockIdx.x & 1u, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const uint32_t row_tiles = p.plan.tiles ? min(p.plan.tiles[0], work.row_tiles) : work.row_tiles;
   const uint32_t tiles = row_tiles * work.column_tiles, k_stages = (p.k + kDepth - 1u) / kDepth;
-  auto place = [&](uint32_t tile) { return place_of(p, tile % row_tiles, work.rows, 1u, tile / row_tiles * 2u * kColumns); };
+  auto place = [&](uint32_t tile) { return place_of(p, tile % row_tiles, work.rows, tile / row_tiles * 2u * kColumns); };
   // rows that a product takes, half of them from either CTA: in boxes of 16 with a plan, otherwise in one of half the most rows
   auto width = [&](const Place& at) { return max((at.end - at.row + 31u) / 32u * 32u, 32u); };
 
