@@ -27,7 +27,7 @@ struct Shape {
   static constexpr uint32_t kScaleColumns = kStageWords * 8;
   static constexpr uint32_t kUsedColumns = NT + 2 * kScaleColumns;
   static constexpr uint32_t kTmemColumns = kUsedColumns <= 128 ? 128 : 256;
-  static constexpr uint32_t kHolder = (3 * kStages + 1) * 8;  // behind the ring: barriers, tensor memory's address, abort flag
+  static constexpr uint32_t kHolder = (3 * kStages + 2) * 8;  // behind the ring: barriers, tensor memory's address, abort flag
   static constexpr uint32_t kBehind = kHolder + 8;
   static constexpr uint32_t kPiece = NT == 16 ? 16 : 32;
 };
@@ -63,6 +63,7 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
   unsigned char* base_pointer = shared_raw + (base - smem_u32(shared_raw));
   const uint32_t behind = work.stages * Z::kStageBytes;
   const uint32_t full = base + behind, scales_full = full + Z::kStages * 8, empty = scales_full + Z::kStages * 8, sums_full = empty + Z::kStages * 8;
+  const uint32_t drained = sums_full + 8;
   const uint32_t joined = base + behind + Z::kBehind;
   volatile uint32_t* holder = reinterpret_cast<volatile uint32_t*>(base_pointer + behind + Z::kHolder);
   volatile uint32_t* abort_flag = holder + 1;
@@ -80,6 +81,7 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         barrier_init(empty + s * 8, 1);  // one tcgen05.commit
       }
       barrier_init(sums_full, 1);  // one tcgen05.commit
+      barrier_init(drained, 1);    // the same, where a CTA gives up
       *abort_flag = 0u;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -196,7 +198,12 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
       __syncwarp();
       if (++s == work.stages) s = 0, phase ^= 1u;
     }
-    if (!ok) give_up();
+    if (!ok) {
+      give_up();
+      if (elect_one()) mma_commit(drained);  // the products already issued read the ring
+      __syncwarp();
+      warp_wait(drained, 0u);
+    }
   } else {
     const uint32_t group = warp - 2u, last_mask = last_word_mask(p.k);
     bool ok = true;
@@ -308,7 +315,7 @@ int run(const KernelArgs& args, const Problem& p, uint32_t row_tiles) {
   CUtensorMap map_w, map_x;
   LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.box_rows), "tensor map was refused");
   auto kernel = stream_kernel<NT, S>;
-  LLMOPT_REQUIRE((allow_shared<kMostShared, stream_kernel<NT, S>>()), "shared memory request was refused");
+  LLMOPT_REQUIRE(allow_shared(kernel, kMostShared), "shared memory request was refused");
   const dim3 grid((uint32_t)tiles * work.splits);
   if (work.splits == 1u)
     launch_kernel(args, kernel, grid, dim3(kThreads), shared_bytes<NT>(work), map_w, map_x, p, work, context_device_error(args.ctx));

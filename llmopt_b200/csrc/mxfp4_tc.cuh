@@ -7,8 +7,6 @@
 #pragma once
 #include <cuda.h>
 
-#include <atomic>
-
 #include "mxfp4.cuh"
 #include "w4a16_tc_device.cuh"
 
@@ -210,20 +208,12 @@ inline bool make_map(CUtensorMap* map, const void* codes, uint64_t k, uint64_t r
 }
 
 
-// Lets a kernel have BYTES of shared memory, the most that any launch of it asks for; said once per device.
-template <uint32_t BYTES, auto KERNEL>
-bool allow_shared() {
-  static std::atomic<uint64_t> said{0};
-  int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess) return false;
-  const uint64_t bit = (uint64_t)1 << (device & 63);
-  if (said.load(std::memory_order_relaxed) & bit) return true;
-  if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES) != cudaSuccess) {
-    cudaGetLastError();
-    return false;
-  }
-  said.fetch_or(bit, std::memory_order_relaxed);
-  return true;
+// Lets a kernel have as much shared memory as any launch of it asks for: the limit is one per kernel, whoever launches it.
+template <typename... Params>
+bool allow_shared(void (*kernel)(Params...), uint32_t bytes) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess) return true;
+  cudaGetLastError();
+  return false;
 }
 
 inline uint32_t most_plan_tiles(uint32_t slots, uint32_t experts) { return slots / kExpertTile + (slots < experts ? slots : experts); }

@@ -312,7 +312,7 @@ int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
   LLMOPT_REQUIRE(tiles < (1u << 28), "too many tiles");
   CUtensorMap map_w, map_x;
   LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.box_rows), "tensor map was refused");
-  LLMOPT_REQUIRE((allow_shared<kSharedBytes, tiles_kernel<S>>()), "shared memory request was refused");
+  LLMOPT_REQUIRE(allow_shared(tiles_kernel<S>, kSharedBytes), "shared memory request was refused");
   launch_cluster_kernel(args, tiles_kernel<S>, dim3(2u * (tiles < pairs ? (uint32_t)tiles : pairs)), dim3(kThreads), kSharedBytes, 2u, map_w, map_x, p,
                         work, context_device_error(args.ctx));
   return check_launch(args);

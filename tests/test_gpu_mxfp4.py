@@ -218,6 +218,58 @@ def test_one_block_at_a_time_meets_its_exponents(runtime):
         assert np.array_equal(read(y), want[:m].astype(np.float32))
 
 
+# rows and columns in other numbers than the tiles have, one to several tiles for every pair of SMs, sums shared out over a cluster's CTAs
+SIZES = [(48, 8192, 8192), (17, 4096, 4096), (64, 4096, 14336), (1, 128256, 256), (33, 20000, 512), (65, 9472, 512), (224, 18944, 256), (225, 2560, 1024),
+         (256, 14336, 512), (448, 4736, 288), (777, 7168, 256), (1000, 1000, 1000 // 32 * 32), (3000, 600, 128), (90, 40, 16384)]
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_linear_in_every_number_of_tiles(runtime, m, n, k):
+    """Values of few bits, whose sums are whole numbers that fp32 holds: exact, whatever adds them in which order."""
+    from llmopt_b200 import dispatch
+
+    rng = np.random.default_rng(m + n + k)
+    pick = np.array([0, 2, 4, 5, 10, 12, 13], np.uint8)  # 0, 1, 2, 3, -1, -2, -3
+    x = rng.choice(pick, (m, k)), np.full((m, k // 32), 127, np.uint8)
+    w = rng.choice(pick, (n, k)), rng.integers(127, 129, (n, k // 32)).astype(np.uint8)
+    want = (mx.values(*x).astype(np.float32) @ mx.values(*w).astype(np.float32).T).astype(np.float32)  # below 2^24, so exact too
+    xt, wt = upload(runtime, x, 255), upload(runtime, w, 255)
+    y = blank(runtime, (m, n), "float32", 256)
+    dispatch.dispatch_mxfp4_linear(context(runtime), input=xt[0], input_scales=xt[1], weight=wt[0], weight_scales=wt[1], output=y)
+    got = read(y, 256)
+    assert np.array_equal(got, want), np.argwhere(got != want)[:5]
+    half = blank(runtime, (m, n), "float16", 256)
+    dispatch.dispatch_mxfp4_linear(context(runtime), input=xt[0], input_scales=xt[1], weight=wt[0], weight_scales=wt[1], output=half)
+    assert np.array_equal(read(half, 256), to_bits(want, "float16").view(np.uint16))
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_products_at_the_ends_of_the_exponents(runtime, m):
+    """One product per sum: exact wherever fp32 holds it, subnormal numbers and infinity included.  A product of two elements has at most four
+    significant bits, so fp32 fails to hold it only below 2^-126, where its numbers lie 2^-149 apart; the tensor cores cut a sum to one of
+    them (as they do its last bits anywhere), so there the result is off by less than 2^-149."""
+    from llmopt_b200 import dispatch
+
+    pairs = [(254, 127), (254, 0), (254, 254), (0, 0), (0, 127), (60, 64), (50, 50), (40, 70), (63, 65), (254, 129), (253, 128), (1, 126), (0, 128)]
+    n, k = 130, 64
+    codes = np.arange(1, 8, dtype=np.uint8)
+    for sx, sw in pairs:
+        x = np.zeros((m, k), np.uint8), np.full((m, 2), 127, np.uint8)
+        w = np.zeros((n, k), np.uint8), np.full((n, 2), 127, np.uint8)
+        x[0][:, 5], x[1][:, 0] = np.resize(codes, m), sx
+        w[0][:, 5], w[1][:, 0] = np.resize(codes[::-1], n), sw
+        w[0][::2, 5] |= 8
+        exact = mx.values(*x) @ mx.values(*w).T
+        with np.errstate(over="ignore"):
+            want = exact.astype(np.float32)
+        held = np.isinf(want) | (want == exact)
+        xt, wt, y = upload(runtime, x), upload(runtime, w), blank(runtime, (m, n), "float32")
+        dispatch.dispatch_mxfp4_linear(context(runtime), input=xt[0], input_scales=xt[1], weight=wt[0], weight_scales=wt[1], output=y)
+        got = read(y)
+        assert np.array_equal(got[held], want[held]), (sx, sw)
+        assert (np.abs(got.astype(np.float64) - exact)[~held] < 2.0 ** -149).all(), (sx, sw)
+
+
 @pytest.mark.parametrize("m,n,k", [(3, 200, 416), (40, 130, 4096), (300, 260, 1024)])
 def test_blocks_of_nan_reach_their_row_or_column_alone(runtime, m, n, k):
     from llmopt_b200 import dispatch
