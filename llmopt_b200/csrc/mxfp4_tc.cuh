@@ -120,37 +120,46 @@ __device__ __forceinline__ void store_rows(const Problem& p, uint32_t row, uint3
 
 constexpr uint32_t kStagingRow = 80, kStagingBytes = 32 * kStagingRow;  // a warp's 32 rows of 64 bytes and 16 of padding
 
-// The same of 16 or 32 rows from `row` on and the warp's 32 columns, through the warp's staging: lanes share the 64 bytes of a row.
+template <Store S> constexpr bool kPaired = S == kStorePairHalf || S == kStorePairBf16;
+
+// Results of sixteen bits of 16 or 32 rows from `row` on and the warp's 32 columns to shared memory, STRIDE bytes a row.
+template <Store S, uint32_t STRIDE, uint32_t COUNT>
+__device__ __forceinline__ void stage_piece(const Problem& p, uint32_t row, uint32_t end, uint32_t column0, const uint32_t (&raw)[COUNT], unsigned char* staging) {
+  typedef typename Element<S>::Type T;
+  const uint32_t lane = threadIdx.x & 31u;
+  if constexpr (kPaired<S>) {
+    const bool odd = lane & 1u;
+    const float scales = row + lane < end ? p.row_scale[row + lane] : 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < COUNT; i += 2) {
+      if (row + i >= end) break;  // the same for the whole warp
+      const uint32_t away = __shfl_xor_sync(0xffffffffu, odd ? raw[i] : raw[i + 1], 1), at = i + (odd ? 1u : 0u);
+      const float scale = __shfl_sync(0xffffffffu, scales, at);
+      const float gate = __uint_as_float(odd ? away : raw[i]) * scale, up = __uint_as_float(odd ? raw[i + 1] : away) * scale;
+      *reinterpret_cast<T*>(staging + at * STRIDE + lane / 2u * 2u) = from_float<T>(silu_short(gate) * up);
+    }
+  } else {
+    const float bias = p.bias && column0 + lane < p.n ? as_float(reinterpret_cast<const T*>(p.bias)[column0 + lane]) : 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < COUNT; ++i) {
+      if (row + i >= end) break;
+      *reinterpret_cast<T*>(staging + i * STRIDE + lane * 2u) = from_float<T>(__uint_as_float(raw[i]) + bias);
+    }
+  }
+}
+
+// The same on their way out: lanes share the 64 bytes (of pairs 32) of a row.
 template <Store S, uint32_t COUNT>
 __device__ __forceinline__ void store_piece(const Problem& p, uint32_t row, uint32_t end, uint32_t column0, const uint32_t (&raw)[COUNT], unsigned char* staging) {
   typedef typename Element<S>::Type T;
-  constexpr bool kPair = S == kStorePairHalf || S == kStorePairBf16;
   const uint32_t lane = threadIdx.x & 31u;
   if constexpr (S == kStoreFloat) {
     store_rows<S>(p, row, end, column0 + lane, raw);
   } else {
-    if constexpr (kPair) {
-      const bool odd = lane & 1u;
-      const float scales = row + lane < end ? p.row_scale[row + lane] : 0.0f;
-#pragma unroll
-      for (uint32_t i = 0; i < COUNT; i += 2) {
-        if (row + i >= end) break;  // the same for the whole warp
-        const uint32_t away = __shfl_xor_sync(0xffffffffu, odd ? raw[i] : raw[i + 1], 1), at = i + (odd ? 1u : 0u);
-        const float scale = __shfl_sync(0xffffffffu, scales, at);
-        const float gate = __uint_as_float(odd ? away : raw[i]) * scale, up = __uint_as_float(odd ? raw[i + 1] : away) * scale;
-        *reinterpret_cast<T*>(staging + at * kStagingRow + lane / 2u * 2u) = from_float<T>(silu_short(gate) * up);
-      }
-    } else {
-      const float bias = p.bias && column0 + lane < p.n ? as_float(reinterpret_cast<const T*>(p.bias)[column0 + lane]) : 0.0f;
-#pragma unroll
-      for (uint32_t i = 0; i < COUNT; ++i) {
-        if (row + i >= end) break;
-        *reinterpret_cast<T*>(staging + i * kStagingRow + lane * 2u) = from_float<T>(__uint_as_float(raw[i]) + bias);
-      }
-    }
+    stage_piece<S, kStagingRow>(p, row, end, column0, raw, staging);
     __syncwarp();
-    constexpr uint32_t kVectors = kPair ? 2 : 4;  // of a row
-    const uint32_t columns = kPair ? p.n / 2u : p.n, first = (kPair ? column0 / 2u : column0) + lane % kVectors * 8u;
+    constexpr uint32_t kVectors = kPaired<S> ? 2 : 4;  // of a row
+    const uint32_t columns = kPaired<S> ? p.n / 2u : p.n, first = (kPaired<S> ? column0 / 2u : column0) + lane % kVectors * 8u;
     const bool vectors = columns % 8u == 0 && ((uintptr_t)p.out & 15u) == 0;
 #pragma unroll
     for (uint32_t i = 0; i < COUNT * kVectors / 32; ++i) {
@@ -190,8 +199,9 @@ __device__ __forceinline__ uint32_t last_word_mask(uint32_t k) {
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// Codes [rows, k / 2] read in boxes of 128 bytes x `box_rows` with the 128-byte swizzle; absent bytes read zero.
-inline bool make_map(CUtensorMap* map, const void* codes, uint64_t k, uint64_t rows, uint32_t box_rows) {
+// Rows of `inner` elements in boxes of box_inner x box_rows.
+inline bool make_map(CUtensorMap* map, CUtensorMapDataType type, uint32_t size, const void* base, uint64_t inner, uint64_t rows, uint32_t box_inner,
+                     uint32_t box_rows, CUtensorMapSwizzle swizzle) {
   static EncodeTiled encode = []() -> EncodeTiled {
     void* pointer = nullptr;
     cudaDriverEntryPointQueryResult result;
@@ -201,12 +211,15 @@ inline bool make_map(CUtensorMap* map, const void* codes, uint64_t k, uint64_t r
     return reinterpret_cast<EncodeTiled>(pointer);
   }();
   if (encode == nullptr) return false;
-  const cuuint64_t dims[2] = {k / 2, rows}, strides[1] = {k / 2};
-  const cuuint32_t box[2] = {kRowBytes, box_rows}, element_strides[2] = {1, 1};
-  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint64_t dims[2] = {inner, rows}, strides[1] = {inner * size};
+  const cuuint32_t box[2] = {box_inner, box_rows}, element_strides[2] = {1, 1};
+  return encode(map, type, 2, const_cast<void*>(base), dims, strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-
+// Codes [rows, k / 2] read in boxes of 128 bytes x `box_rows` with the 128-byte swizzle; absent bytes read zero.
+inline bool make_map(CUtensorMap* map, const void* codes, uint64_t k, uint64_t rows, uint32_t box_rows) {
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1u, codes, k / 2, rows, kRowBytes, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
 
 // Lets a kernel have as much shared memory as any launch of it asks for: the limit is one per kernel, whoever launches it.
 template <typename... Params>

@@ -26,7 +26,10 @@ constexpr uint32_t kStageBytes = kInputScalesAt + kStageWords * kInputAtoms * kA
 constexpr uint32_t kStages = 5, kSums = 2;
 constexpr uint32_t kScaleColumns = kStageWords * 4 * (1 + kInputAtoms), kTmemColumns = 512;
 static_assert(kSums * kMostRows + 2 * kScaleColumns <= kTmemColumns && kStageBytes % 1024 == 0, "tensor memory, alignment of tiles");
-constexpr uint32_t kStaging = kStages * kStageBytes, kBarriers = kStaging + kEpilogueWarps * kStagingBytes;
+// of a warp that stores: two boxes of 32 rows of 64 bytes, or the padded rows of store_piece
+constexpr uint32_t kBoxBytes = 32 * 64, kWarpStaging = 2 * kBoxBytes;
+static_assert(kWarpStaging >= kStagingBytes, "staging");
+constexpr uint32_t kStaging = kStages * kStageBytes, kBarriers = kStaging + kEpilogueWarps * kWarpStaging;
 constexpr uint32_t kHolder = kBarriers + (3 * kStages + 2 * kSums + 1) * 8, kAbort = kHolder + 4;
 constexpr uint32_t kSharedBytes = kAbort + 4 + 1024;  // slack: 1024-byte alignment of the tiles
 static_assert(kSharedBytes <= 227 * 1024, "shared memory");
@@ -34,6 +37,7 @@ static_assert(kSharedBytes <= 227 * 1024, "shared memory");
 struct Work {
   uint32_t row_tiles, column_tiles;  // of x, of pairs of weight tiles
   uint32_t rows, box_rows;           // most rows of a tile; rows of a box of x
+  uint32_t boxes;                    // results leave in boxes
 };
 
 // The first CTA's barriers, from either.
@@ -68,10 +72,21 @@ __device__ __forceinline__ void pair_commit(uint32_t bar) {
                : "memory");
 }
 
+// A box of shared memory to the rows and columns of the results it belongs to.
+__device__ __forceinline__ void store_box(const CUtensorMap* map, int32_t x, int32_t y, uint32_t source) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(source) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// Until all but the last BOXES boxes of this thread have been read.
+template <int BOXES>
+__device__ __forceinline__ void await_boxes() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(BOXES) : "memory");
+}
+
 template <Store S>
 __global__ void __launch_bounds__(kThreads, 1)
-tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ Problem p, const Work work,
-             uint32_t* error_word) {
+tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_out,
+             const __grid_constant__ Problem p, const Work work, uint32_t* error_word) {
   extern __shared__ unsigned char shared_raw[];
   grid_chain_prologue();
   const uint32_t base = (smem_u32(shared_raw) + 1023u) & ~1023u;
@@ -251,8 +266,8 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     if (!ok) give_up();
   } else {
     const uint32_t worker = warp - 2u - kScaleWarps, quarter = warp & 3u, side = worker >> 2;  // lanes of tensor memory; every other piece
-    unsigned char* const staging = base_pointer + kStaging + worker * kStagingBytes;
-    uint32_t turn = 0;
+    unsigned char* const staging = base_pointer + kStaging + worker * kWarpStaging;
+    uint32_t turn = 0, turn_of_box = 0;
     bool ok = true;
     for (uint32_t tile = pair; tile < tiles && ok; tile += pairs, ++turn) {
       const uint32_t which = turn % kSums;
@@ -272,13 +287,31 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         uint32_t raw[32];
         tmem_load_32(address + piece * 32u, raw);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        store_piece<S>(p, row, at.end, column, raw, staging);
+        constexpr uint32_t kWidth = kPaired<S> ? 16 : 32;  // columns of results
+        const uint32_t out_column = kPaired<S> ? column / 2u : column, columns = kPaired<S> ? p.n / 2u : p.n;
+        if (S != kStoreFloat && work.boxes && row + 32u <= at.end && out_column + kWidth <= columns) {
+          // whole pieces: one of two boxes is filled while the other is on its way
+          unsigned char* const box = staging + turn_of_box * kBoxBytes;
+          if (lane == 0) await_boxes<1>();
+          __syncwarp();
+          if constexpr (S != kStoreFloat) stage_piece<S, kWidth * 2>(p, row, at.end, column, raw, box);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) store_box(&map_out, (int32_t)out_column, (int32_t)row, smem_u32(box));
+          turn_of_box ^= 1u;
+        } else {
+          if (lane == 0) await_boxes<0>();
+          __syncwarp();
+          store_piece<S>(p, row, at.end, column, raw, staging);
+        }
         __syncwarp();  // tcgen05.ld needs the whole warp
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) first_arrive(first_address(sums_empty + which * 8));
     }
+    if (lane == 0) await_boxes<0>();
+    __syncwarp();
   }
 
   __syncthreads();
@@ -296,7 +329,7 @@ namespace mxfp4 {
 template <Store S>
 int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
   const uint32_t pairs = (uint32_t)context_sm_count(args.ctx) / 2u, k_stages = (p.k + kDepth - 1u) / kDepth;
-  Work work = {plan_tiles, (p.n + 2u * kColumns - 1u) / (2u * kColumns), kExpertTile, 16u};
+  Work work = {plan_tiles, (p.n + 2u * kColumns - 1u) / (2u * kColumns), kExpertTile, 16u, 0u};
   if (!p.plan.tiles) {
     // the height with the shortest estimate: rounds of tiles times the cycles of one, of which a stage takes about 280 and one per row
     uint64_t least = ~0ull;
@@ -312,8 +345,15 @@ int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
   LLMOPT_REQUIRE(tiles < (1u << 28), "too many tiles");
   CUtensorMap map_w, map_x;
   LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.box_rows), "tensor map was refused");
+  CUtensorMap map_out = map_x;  // not read without boxes
+  const uint32_t columns = kPaired<S> ? p.n / 2u : p.n;
+  if (S != kStoreFloat && columns % 8u == 0 && ((uintptr_t)p.out & 15u) == 0) {
+    const bool half = sizeof(typename Element<S>::Type) == 2 && (S == kStoreHalf || S == kStorePairHalf);
+    work.boxes = make_map(&map_out, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2u, p.out, columns, p.m,
+                          kPaired<S> ? 16u : 32u, 32u, CU_TENSOR_MAP_SWIZZLE_NONE);
+  }
   LLMOPT_REQUIRE(allow_shared(tiles_kernel<S>, kSharedBytes), "shared memory request was refused");
-  launch_cluster_kernel(args, tiles_kernel<S>, dim3(2u * (tiles < pairs ? (uint32_t)tiles : pairs)), dim3(kThreads), kSharedBytes, 2u, map_w, map_x, p,
+  launch_cluster_kernel(args, tiles_kernel<S>, dim3(2u * (tiles < pairs ? (uint32_t)tiles : pairs)), dim3(kThreads), kSharedBytes, 2u, map_w, map_x, map_out, p,
                         work, context_device_error(args.ctx));
   return check_launch(args);
 }
