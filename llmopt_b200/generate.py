@@ -1,7 +1,7 @@
 """Generates token ids from a model folder (config.json and model.safetensors):
 
   python -m llmopt_b200.generate --model DIR --prompt 5,17,3 [--prompt 8,1] [--tokens 32] [--batch 4]
-         [--temperature 0.8 --top-k 40 --top-p 0.95 --min-p 0.05 --seed 1] [--stop 2] [--dtype bfloat16|float32]
+         [--temperature 0.8 --top-k 40 --top-p 0.95 --min-p 0.05 --seed 1] [--stop 2] [--dtype bfloat16|float32] [--experts mxfp4]
 
 One line of ids per prompt.  Tokenizers are outside this library: prompts and results are ids."""
 
@@ -25,6 +25,7 @@ def main(argv=None) -> None:
     parser.add_argument("--tokens", type=int, default=32, help="most tokens to generate after a prompt")
     parser.add_argument("--batch", type=int, default=8, help="most sequences that decode side by side")
     parser.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    parser.add_argument("--experts", default=None, choices=["mxfp4"], help="format of routed experts' weights (default: --dtype)")
     parser.add_argument("--temperature", type=float, default=0.0)
     parser.add_argument("--top-k", type=int, default=0)
     parser.add_argument("--top-p", type=float, default=0.0)
@@ -34,7 +35,8 @@ def main(argv=None) -> None:
     args = parser.parse_args(argv)
     config, weights = load_model(args.model)
     capacity = max(len(prompt) for prompt in args.prompt) + args.tokens
-    engine = create_engine(Runtime(), config, weights, batch=min(args.batch, len(args.prompt)), capacity=capacity, dtype=args.dtype)
+    options = {"experts": args.experts} if args.experts else {}
+    engine = create_engine(Runtime(), config, weights, batch=min(args.batch, len(args.prompt)), capacity=capacity, dtype=args.dtype, **options)
     for tokens in engine.generate(args.prompt, args.tokens, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
                                   min_p=args.min_p, seed=args.seed, stop=args.stop):
         print(",".join(map(str, tokens)), flush=True)

@@ -17,10 +17,11 @@ import numpy as np
 
 from . import parameters
 from .cuda_native import Batch, Buffer, DispatchItem, Prebaked, Runtime, pack_records, sample_f32
-from .feed_forward import FEED_FORWARDS
+from .dispatch import Context, Tensor, dispatch_mxfp4_quantize, mxfp4_scale_words
+from .feed_forward import FEED_FORWARDS, RoutedExpertsMxfp4
 from .kv_cache import RowLayout, RowRegion, SequenceTable
 from .mixers import LayerMixer, Step, attention_specs
-from .model import AttentionSpec, MixerConfig
+from .model import AttentionSpec, ExpertsSpec, MixerConfig
 from .quantize import rotary_pairs
 from .residual import RESIDUALS
 from .safetensors_archive import as_bfloat16_bits, as_float32
@@ -50,7 +51,9 @@ class _Layer:
         self.mixer = LayerMixer(engine, layer.mixer, weights, f"{prefix}.mix", index)
         self.feed_forward = None
         if layer.feed_forward:
-            self.feed_forward = FEED_FORWARDS[type(layer.feed_forward)](engine, layer.feed_forward, weights, f"{prefix}.mlp")
+            quantized = engine.experts == "mxfp4" and isinstance(layer.feed_forward, ExpertsSpec)
+            build = RoutedExpertsMxfp4 if quantized else FEED_FORWARDS[type(layer.feed_forward)]
+            self.feed_forward = build(engine, layer.feed_forward, weights, f"{prefix}.mlp")
         if engine.config.token_side:
             self.side_gate, self.side_proj = (engine.upload_matrix(weights[f"{prefix}.side.{name}"]) for name in ("gate", "proj"))
             self.side_norm = engine.upload_vector(weights[f"{prefix}.side.norm"])
@@ -85,13 +88,20 @@ class _Plan:
 class MixerEngine:
     def __init__(self, runtime: Runtime, config: MixerConfig, weights, *, batch: int = 1, capacity: int = 1024,
                  sequences: Optional[int] = None, token_capacity: Optional[int] = None, page: int = 16,
-                 dtype: str = "bfloat16", prompt_rows: int = 2048):
+                 dtype: str = "bfloat16", prompt_rows: int = 2048, experts: Optional[str] = None):
         """``batch``: sequences ``step`` decodes side by side; ``capacity``: most tokens of a sequence;
         ``sequences``: live sequences at most (default ``batch``); ``token_capacity``: token slots they
         share (default: all of them at full length); ``prompt_rows``: rows of a prompt that run at
-        once, longer ones run in portions."""
+        once, longer ones run in portions; ``experts``: "mxfp4" holds routed experts' matrices in microscaled 4-bit
+        floating point, quantized here, and quantizes what they read (bfloat16 models whose widths are whole blocks of 32)."""
         if dtype not in ("bfloat16", "float32"):
             raise ValueError(f"unsupported element type: {dtype}")
+        if experts not in (None, "mxfp4"):
+            raise ValueError(f"unsupported format of experts: {experts}")
+        routed = [layer.feed_forward for layer in config.layers if isinstance(layer.feed_forward, ExpertsSpec)]
+        if experts and (dtype != "bfloat16" or not routed or any(size % 32 for spec in routed for size in (spec.width, config.width))):
+            raise ValueError("MXFP4 experts need a bfloat16 model with routed experts whose widths are multiples of 32")
+        self.experts = experts
         self.runtime, self.config, self.batch, self.capacity = runtime, config, batch, capacity
         self.suffix, self.itemsize = ("bf16", 2) if dtype == "bfloat16" else ("f32", 4)
         self.max_rows = max(min(prompt_rows, capacity), batch)
@@ -125,6 +135,15 @@ class MixerEngine:
     def upload_matrix(self, array) -> Buffer:
         """A weight matrix in the model's element type."""
         return Buffer.of_array(self.runtime, as_bfloat16_bits(array) if self.itemsize == 2 else as_float32(array))
+
+    def upload_matrix_mxfp4(self, array) -> Tuple[Buffer, Buffer]:
+        """A weight matrix in MXFP4: codes and exponents, quantized on the device from bfloat16."""
+        rows, k = array.shape
+        held = Tensor(self.upload_matrix(array), (rows, k), "bfloat16")
+        codes, scales = self.empty_bytes(rows * k // 2), self.empty_bytes(mxfp4_scale_words(k) * rows * 4)
+        dispatch_mxfp4_quantize(Context(self.runtime), input=held, codes=Tensor(codes, (rows, k // 2), "uint8"),
+                                scales=Tensor(scales, (mxfp4_scale_words(k), rows), "uint32"))
+        return codes, scales
 
     def upload_vector(self, array) -> Buffer:
         """Norm weights, biases and the like, fp32 in every model."""

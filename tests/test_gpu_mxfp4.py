@@ -442,6 +442,103 @@ def test_a_routed_layer_in_one_batch(runtime, rows, experts, top, width, inner):
         check(y_got[mine], want, allowed(hidden_v[mine], w, want, "float32"))
 
 
+def routed_model(experts=6, top=2, inner=64, width=96):
+    from mixer_models import dense_mlp, routed_mlp, sandwich_config, weights_of, window_layer
+
+    config = sandwich_config([window_layer(mlp=routed_mlp(experts, top, inner)), window_layer(kv_from=0, mlp=dense_mlp(64)),
+                              window_layer(mlp=routed_mlp(4, 1, 160))], width=width)
+    return config, weights_of(config, seed=4)
+
+
+@pytest.mark.parametrize("tokens", [1, 7, 60, 300])
+def test_experts_of_a_decoder_in_mxfp4(runtime, tokens):
+    """A prompt through an engine whose experts are quantized, replayed kernel by kernel: each against its own inputs."""
+    from llmopt_b200 import mixer_engine
+    from llmopt_b200.model import parse_config
+
+    config, weights = routed_model()
+    engine = mixer_engine.MixerEngine(runtime, parse_config(config), weights, capacity=320, experts="mxfp4")
+    for index, (spec, inner) in ((0, (6, 64)), (2, (4, 160))):  # matrices as they were quantized
+        feed = engine.layers[index].feed_forward
+        for held, matrix, k in ((feed.up, None, 96), (feed.down, None, inner)):
+            rows = spec * (2 * inner if held is feed.up else 96)
+            name = lambda e, part: weights[f"l{index}.mlp.e{e}.{part}"]
+            source = np.concatenate([np.stack([name(e, "gate"), name(e, "up")], 1).reshape(-1, k) if held is feed.up else name(e, "down")
+                                     for e in range(spec)])
+            nibbles, exponents = mx.quantize(source)
+            assert source.shape == (rows, k) and np.array_equal(np.frombuffer(held[0].contents(), np.uint8)[:rows * k // 2].reshape(rows, -1), mx.pack(nibbles))
+            words = np.frombuffer(held[1].contents(), np.uint32)[:(k + 127) // 128 * rows].reshape(-1, rows)
+            assert np.array_equal(mx.exponents(words, k), exponents)
+    ids = np.random.default_rng(tokens).integers(0, config["vocab"], tokens).tolist()
+    first = engine.prefill(ids)
+    assert first == engine.prefill(ids)
+    plan = mixer_engine._Plan(engine, 1, tokens)
+    engine._record_layers(plan.step)
+    plan.write(ids, [0], [engine._row(0)])
+    seen = []
+
+    def held(buffers, rows, k):
+        codes = np.frombuffer(buffers[0].contents(), np.uint8)[:rows * k // 2].reshape(rows, -1)
+        words = np.frombuffer(buffers[1].contents(), np.uint32)[:(k + 127) // 128 * rows].reshape(-1, rows)
+        return mx.unpack(codes), mx.exponents(words, k)
+
+    for item in plan.items:
+        runtime.dispatch(item.name, buffers=item.buffers, parameters=item.parameters)
+        numbers, b = np.frombuffer(item.parameters, np.uint32).tolist(), item.buffers
+        if item.name.startswith("llmopt_mxfp4_quantize"):
+            rows, k = numbers[:2]
+            x = np.frombuffer(b[0].contents(), np.uint16)
+            if "rows" in item.name:
+                index = np.frombuffer(b[1].contents(), np.uint32)[:rows]
+                x = x[:numbers[3] * k].reshape(-1, k)[index]
+            want = mx.quantize(from_bits(x[:rows * k].reshape(rows, k) if x.ndim == 1 else x, "bfloat16"))
+            got = held(b[-2:], rows, k)
+            assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+        elif item.name.startswith("llmopt_mxfp4_expert_rows"):
+            slots, n, k, experts, paired = numbers
+            xv, wv = mx.values(*held(b[0:2], slots, k)), mx.values(*held(b[2:4], experts * n, k)).reshape(experts, n, k)
+            plan_words = np.frombuffer(b[4].contents(), np.uint32).reshape(-1, 4)
+            covered = 0
+            for expert, begin, end, _ in plan_words[1:1 + plan_words[0, 0]]:
+                sums = xv[begin:end] @ wv[expert].T
+                off = allowed(xv[begin:end], wv[expert], np.zeros(1), "float32")
+                if paired:
+                    score = np.frombuffer(b[5].contents(), np.float32)[begin:end, None].astype(np.float64)
+                    got = from_bits(np.frombuffer(b[6].contents(), np.uint16)[:slots * n // 2].reshape(slots, -1)[begin:end], "bfloat16")
+                    gate, value = sums[:, 0::2] * score, sums[:, 1::2] * score
+                    want = gate / (1 + np.exp(-gate)) * value
+                    check(got, want, 1.1 * off[:, 0::2] * (np.abs(value) + off[:, 1::2]) + np.abs(gate) * off[:, 1::2]
+                          + 2.0 ** -8 * (1 + 2.0 ** -6) * np.abs(want) + 2.0 ** -20 * np.abs(want) + 2.0 ** -25)
+                else:
+                    got = np.frombuffer(b[6].contents(), np.float32)[:slots * n].reshape(slots, n)[begin:end].astype(np.float64)
+                    check(got, sums, off + HALF_STEP["float32"] * np.abs(sums))
+                covered += end - begin
+            assert covered == slots
+        else:
+            continue
+        seen.append(item.name)
+    assert len(seen) == 8
+
+
+def test_generation_with_experts_in_mxfp4(runtime, tmp_path, capsys):
+    """Prompts, steps, chained steps and the command give the same tokens as one another."""
+    from llmopt_b200 import generate, mixer_engine
+    from llmopt_b200.model import parse_config
+    from test_gpu_dalorax import checkpoint
+
+    config, weights = routed_model(experts=8, top=3, inner=32, width=64)
+    engine = mixer_engine.MixerEngine(runtime, parse_config(config), weights, capacity=64, experts="mxfp4")
+    stream = [engine.prefill([3, 99, 41])]
+    for past in range(3, 9):
+        stream += engine.step(stream[-1:], past)
+    engine.prefill([3, 99, 41])
+    chained, _ = engine.generate_chained(stream[:1], 3, 6)
+    assert chained == stream[1:]
+    checkpoint(tmp_path, config, weights)
+    generate.main(["--model", str(tmp_path), "--prompt", "3,99,41", "--tokens", "7", "--experts", "mxfp4"])
+    assert capsys.readouterr().out.splitlines() == [",".join(map(str, stream))]
+
+
 def test_a_layer_replayed_as_a_plan(runtime):
     """Quantization and product in a plan that is replayed with new inputs."""
     from llmopt_b200 import dispatch, parameters

@@ -143,3 +143,36 @@ def test_entry_points_need_a_context():
     thread.start()
     thread.join()
     assert got == [1, 1, 1, 1, b"CUDA context has been finalized"]
+
+
+# ---- routed experts of a decoder ------------------------------------------------------------------------
+
+def test_records_of_a_step_with_experts_in_mxfp4():
+    """Any number of rows goes the same way: sorted, quantized, multiplied, quantized, multiplied, combined."""
+    from unittest import mock
+
+    from llmopt_b200 import mixer_engine
+    from mixer_models import dense_mlp, routed_mlp, sandwich_config, window_layer
+    from test_dalorax_cpu import RecordingEngine
+
+    config = sandwich_config([window_layer(mlp=dense_mlp(64)), window_layer(kv_from=0, mlp=routed_mlp(6, 2, 32))], width=96)
+    with mock.patch.object(mixer_engine.MixerEngine, "upload_matrix_mxfp4", lambda self, array: (array.shape, "scales")):
+        engine = RecordingEngine(config, batch=3, capacity=256, experts="mxfp4")
+    assert engine.layers[1].feed_forward.up == ((6 * 2 * 32, 96), "scales") and engine.layers[1].feed_forward.down == ((6 * 96, 32), "scales")
+    routed = ["llmopt_route_rows_f32", "llmopt_route_plan", "llmopt_mxfp4_quantize_rows_bf16", "llmopt_mxfp4_expert_rows_bf16",
+              "llmopt_mxfp4_quantize_bf16", "llmopt_mxfp4_expert_rows_bf16", "llmopt_expert_combine_bf16"]
+    for recorded in engine.names.values():
+        assert recorded[-7:] == routed and not any("mxfp4" in name for name in recorded[:-7])
+
+
+def test_experts_in_mxfp4_need_whole_blocks_and_bfloat16():
+    from mixer_models import dense_mlp, routed_mlp, sandwich_config, window_layer
+    from test_dalorax_cpu import RecordingEngine
+
+    routed = [window_layer(mlp=routed_mlp(4, 2, 32))]
+    for config, options in ((sandwich_config(routed, width=104), {}), (sandwich_config([window_layer(mlp=routed_mlp(4, 2, 48))], width=96), {}),
+                            (sandwich_config(routed, width=96), {"dtype": "float32"}), (sandwich_config([window_layer(mlp=dense_mlp(64))], width=96), {})):
+        with pytest.raises(ValueError, match="multiples of 32"):
+            RecordingEngine(config, capacity=64, experts="mxfp4", **options)
+    with pytest.raises(ValueError, match="unsupported format"):
+        RecordingEngine(sandwich_config(routed, width=96), capacity=64, experts="int4")
