@@ -17,26 +17,30 @@ namespace llmopt {
 namespace {
 using namespace mxfp4;
 
-constexpr uint32_t kAhead = 4, kDepth = kBoxDepth, kStageWords = kDepth / kWordValues;  // of a stage
+constexpr uint32_t kDepth = 512, kBoxes = kDepth / kBoxDepth, kStageWords = kDepth / kWordValues;  // of a stage
+constexpr uint32_t kAhead = 3;  // stages of exponents that are under way in registers
+static_assert(kStageWords == kScaleWarps, "a warp per word of a stage");
 constexpr uint32_t kMostRows = 224, kLoneRows = 256, kInputAtoms = 2;  // of a tile; of the only one of every pair
 constexpr uint32_t kEpilogueWarps = 8, kThreads = (2 + kScaleWarps + kEpilogueWarps) * 32;
-constexpr uint32_t kWeightBytes = kColumns * kRowBytes, kInputBytes = kLoneRows / 2 * kRowBytes;
-constexpr uint32_t kScalesAt = kWeightBytes + kInputBytes, kInputScalesAt = kScalesAt + kStageWords * kAtom;
-constexpr uint32_t kStageBytes = kInputScalesAt + kStageWords * kInputAtoms * kAtom;
-constexpr uint32_t kStages = 5, kSums = 2;
-constexpr uint32_t kScaleColumns = kStageWords * 4 * (1 + kInputAtoms), kTmemColumns = 512;
-static_assert(kSums * kMostRows + 2 * kScaleColumns <= kTmemColumns && kStageBytes % 1024 == 0, "tensor memory, alignment of tiles");
-// of a warp that stores: two boxes of 32 rows of 64 bytes, or the padded rows of store_piece
-constexpr uint32_t kBoxBytes = 32 * 64, kWarpStaging = 2 * kBoxBytes;
-static_assert(kWarpStaging >= kStagingBytes, "staging");
-constexpr uint32_t kStaging = kStages * kStageBytes, kBarriers = kStaging + kEpilogueWarps * kWarpStaging;
-constexpr uint32_t kHolder = kBarriers + (3 * kStages + 2 * kSums + 1) * 8, kAbort = kHolder + 4;
-constexpr uint32_t kSharedBytes = kAbort + 4 + 1024;  // slack: 1024-byte alignment of the tiles
-static_assert(kSharedBytes <= 227 * 1024, "shared memory");
+constexpr uint32_t kBoxBytes = kColumns * kRowBytes;  // of weights
+// A stage: codes of weights, exponents of weights and of x, codes of x, of as many rows as the launch's tiles have, which says how many
+// stages there are.
+constexpr uint32_t kScalesAt = kBoxes * kBoxBytes, kInputScalesAt = kScalesAt + kStageWords * kAtom;
+constexpr uint32_t kInputAt = kInputScalesAt + kStageWords * kInputAtoms * kAtom;
+constexpr uint32_t kMostStages = 4, kSums = 2;
+constexpr uint32_t kWordColumns = 4 * (1 + kInputAtoms), kScaleColumns = kStageWords * kWordColumns, kTmemColumns = 512;
+static_assert(kSums * kMostRows + kScaleColumns <= kTmemColumns && kInputAt % 1024 == 0, "tensor memory, alignment of tiles");
+// In front of the ring: barriers, tensor memory's address, abort flag, and the staging of the warps that store, which lies over the ring where
+// no pair has a second tile that would be on its way into it.
+constexpr uint32_t kHolder = (3 * kMostStages + 2 * kSums + 1) * 8, kAbort = kHolder + 4, kFront = 1024, kMostShared = 227 * 1024;
+constexpr uint32_t kStaging = kEpilogueWarps * kStagingBytes;
+static_assert(kAbort + 4 <= kFront && kStaging % 1024 == 0, "alignment of tiles");
+static_assert(kStagingBytes >= 32 * 64, "a box of results");
 
 struct Work {
   uint32_t row_tiles, column_tiles;  // of x, of pairs of weight tiles
-  uint32_t rows, box_rows;           // most rows of a tile; rows of a box of x
+  uint32_t rows;                     // most of a tile; either CTA copies half of them, whatever there are
+  uint32_t stages, stage_bytes, ring;
   uint32_t boxes;                    // results leave in boxes
 };
 
@@ -77,11 +81,8 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, int32_t x, int
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(source) : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// Until all but the last BOXES boxes of this thread have been read.
-template <int BOXES>
-__device__ __forceinline__ void await_boxes() {
-  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(BOXES) : "memory");
-}
+// Until this thread's boxes have been read.
+__device__ __forceinline__ void await_box() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
 template <Store S>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -91,19 +92,20 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
   grid_chain_prologue();
   const uint32_t base = (smem_u32(shared_raw) + 1023u) & ~1023u;
   unsigned char* base_pointer = shared_raw + (base - smem_u32(shared_raw));
-  const uint32_t full = base + kBarriers, scales_full = full + kStages * 8, empty = scales_full + kStages * 8;
-  const uint32_t sums_full = empty + kStages * 8, sums_empty = sums_full + kSums * 8, drained = sums_empty + kSums * 8;
+  const uint32_t full = base, scales_full = full + kMostStages * 8, empty = scales_full + kMostStages * 8;
+  const uint32_t sums_full = empty + kMostStages * 8, sums_empty = sums_full + kSums * 8, drained = sums_empty + kSums * 8;
   volatile uint32_t* holder = reinterpret_cast<volatile uint32_t*>(base_pointer + kHolder);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(base_pointer + kAbort);
   const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u, rank = blockIdx.x & 1u, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const uint32_t row_tiles = p.plan.tiles ? min(p.plan.tiles[0], work.row_tiles) : work.row_tiles;
   const uint32_t tiles = row_tiles * work.column_tiles, k_stages = (p.k + kDepth - 1u) / kDepth;
   auto place = [&](uint32_t tile) { return place_of(p, tile % row_tiles, work.rows, tile / row_tiles * 2u * kColumns); };
-  // rows that a product takes, half of them from either CTA: in boxes of 16 with a plan, otherwise in one of half the most rows
+  const uint32_t half_bytes = work.rows / 2u * kRowBytes;
+  // rows that a product takes, half of them from either CTA
   auto width = [&](const Place& at) { return max((at.end - at.row + 31u) / 32u * 32u, 32u); };
 
   if (threadIdx.x == 0) {
-    for (uint32_t s = 0; s < kStages; ++s) {
+    for (uint32_t s = 0; s < work.stages; ++s) {
       barrier_init(full + s * 8, 1);  // of the first CTA, for both: its expect_tx arrival; completes by byte count
       barrier_init(scales_full + s * 8, 2 * kScaleWarps);  // the same
       barrier_init(empty + s * 8, 1);  // one tcgen05.commit
@@ -135,10 +137,9 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     bool ok = true;
     for (uint32_t tile = pair; tile < tiles && ok; tile += pairs) {
       const Place at = place(tile);
-      const uint32_t half = uniform(width(at)) / 2u, x_row = uniform(at.row) + rank * half, w_row = uniform(at.w_row) + rank * kColumns;
-      const uint32_t boxes = p.plan.tiles ? half / work.box_rows : 1u;
+      const uint32_t x_row = uniform(at.row + rank * (width(at) / 2u)), w_row = uniform(at.w_row) + rank * kColumns;
       for (uint32_t ks = 0; ks < k_stages; ++ks, ++issued) {
-        const uint32_t stage = base + s * kStageBytes;
+        const uint32_t stage = base + work.ring + s * work.stage_bytes, boxes = min(kBoxes, (p.k - ks * kDepth + kBoxDepth - 1u) / kBoxDepth);
         ok = !*abort_flag && warp_wait(empty + s * 8, phase);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) {
@@ -147,60 +148,63 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         }
         if (elect_one()) {
           const uint32_t first = first_address(full + s * 8);
-          if (rank == 0u) barrier_expect_tx(full + s * 8, 2u * (kWeightBytes + boxes * work.box_rows * kRowBytes));
-          pair_load(stage, &map_w, (int32_t)(ks * kRowBytes), (int32_t)w_row, first);
-          for (uint32_t box = 0; box < boxes; ++box)
-            pair_load(stage + kWeightBytes + box * work.box_rows * kRowBytes, &map_x, (int32_t)(ks * kRowBytes), (int32_t)(x_row + box * work.box_rows), first);
+          if (rank == 0u) barrier_expect_tx(full + s * 8, 2u * boxes * (kBoxBytes + half_bytes));
+          for (uint32_t box = 0; box < boxes; ++box) {
+            const int32_t x = (int32_t)((ks * kBoxes + box) * kRowBytes);
+            pair_load(stage + box * kBoxBytes, &map_w, x, (int32_t)w_row, first);
+            pair_load(stage + kInputAt + box * half_bytes, &map_x, x, (int32_t)x_row, first);
+          }
         }
         __syncwarp();
-        if (++s == kStages) s = 0, phase ^= 1u;
+        if (++s == work.stages) s = 0, phase ^= 1u;
       }
     }
     // on the way out after a failure the copies already started must land first: both CTAs' have when the first one's barriers say so
     if (rank == 0u && (!ok || *abort_flag))
-      for (uint32_t i = issued > kStages ? issued - kStages : 0u; i < issued; ++i) barrier_wait(full + (i % kStages) * 8, (i / kStages) & 1u);
+      for (uint32_t i = issued > work.stages ? issued - work.stages : 0u; i < issued; ++i)
+        barrier_wait(full + (i % work.stages) * 8, (i / work.stages) & 1u);
     __syncwarp();
   } else if (warp == 1 && rank == 1u) {
     // the first CTA issues for both
   } else if (warp == 1) {
-    uint32_t s = 0, phase = 0, buffer = 0, turn = 0;
+    uint32_t s = 0, phase = 0, turn = 0;
     bool ok = true;
     for (uint32_t tile = pair; tile < tiles && ok; tile += pairs, ++turn) {
       const uint32_t rows = uniform(width(place(tile)));
       const uint32_t low = mxf4_instruction(2u * kColumns, rows, 0u), high = mxf4_instruction(2u * kColumns, rows, 1u);
-      const uint32_t which = turn % kSums, sums = tmem_base + which * kMostRows;
+      const uint32_t which = turn % kSums, sums = tmem_base + which * kMostRows, scales = tmem_base + kSums * kMostRows;
       ok = !*abort_flag && warp_wait(sums_empty + which * 8, ((turn / kSums) & 1u) ^ 1u);
       ok = __all_sync(0xffffffffu, ok);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       for (uint32_t ks = 0; ks < k_stages && ok; ++ks) {
-        const uint32_t stage = base + s * kStageBytes;
+        const uint32_t stage = base + work.ring + s * work.stage_bytes;
         ok = !*abort_flag && warp_wait(full + s * 8, phase) && warp_wait(scales_full + s * 8, phase);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t scales = tmem_base + kSums * kMostRows + buffer * kScaleColumns, left = p.k - ks * kDepth;
-        const uint64_t a = operand_descriptor(stage), b = operand_descriptor(stage + kWeightBytes);
+        const uint32_t left = p.k - ks * kDepth;
+        const uint64_t a = operand_descriptor(stage), b = operand_descriptor(stage + kInputAt);
         if (elect_one()) {
 #pragma unroll
           for (uint32_t g = 0; g < kStageWords; ++g) {
             if (g * kWordValues >= left) break;
-            const uint32_t columns = scales + g * 4u * (1u + kInputAtoms), atoms = stage + kInputScalesAt + g * kInputAtoms * kAtom;
+            const uint32_t columns = scales + g * kWordColumns, atoms = stage + kInputScalesAt + g * kInputAtoms * kAtom;
             pair_copy_atom(columns, stage + kScalesAt + g * kAtom);
             pair_copy_atom(columns + 4u, atoms);
             if (rows > 128u) pair_copy_atom(columns + 8u, atoms + kAtom);
-          }
 #pragma unroll
-          for (uint32_t j = 0; j < kDepth / 64; ++j) {
-            if (j * 64u >= left) break;
-            const uint32_t columns = scales + j / 2u * 4u * (1u + kInputAtoms);
-            pair_mma(sums, a + j * 2u, b + j * 2u, j & 1u ? high : low, columns, columns + 4u, (ks > 0 || j > 0) ? 1u : 0u);
+            for (uint32_t j = 0; j < 2; ++j) {
+              if (g * kWordValues + j * 64u >= left) break;
+              const uint32_t box = g / 2u, at_box = (g % 2u * 2u + j) * 2u;  // 32 bytes of the box's rows, in the descriptor's 16
+              pair_mma(sums, a + box * (kBoxBytes / 16u) + at_box, b + box * (half_bytes / 16u) + at_box, j ? high : low, columns, columns + 4u,
+                       (ks > 0 || g > 0 || j > 0) ? 1u : 0u);
+            }
           }
           pair_commit(empty + s * 8);
           if (ks + 1u == k_stages) pair_commit(sums_full + which * 8);
         }
         __syncwarp();
-        buffer ^= 1u;
-        if (++s == kStages) s = 0, phase ^= 1u;
+        if (++s == work.stages) s = 0, phase ^= 1u;
       }
     }
     if (!ok) {
@@ -212,26 +216,29 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       warp_wait(drained, 0u);
     }
   } else if (warp < 2u + kScaleWarps) {
-    // the words of a group of a stage: of the CTA's weight rows, or of the tile's rows of x, lane, lane + 32, ...
-    const uint32_t group = (warp - 2u) % kStageWords, words = words_of(p.k), last_mask = last_word_mask(p.k);
-    const bool of_x = warp - 2u >= kStageWords;
-    constexpr uint32_t kWords = kLoneRows / 32;
-    uint32_t held[kAhead][kWords];
+    // the words of group warp - 2 of a stage, of the CTA's weight rows and of the tile's rows of x: lane, lane + 32, ...
+    const uint32_t group = warp - 2u, words = words_of(p.k), last_mask = last_word_mask(p.k);
+    uint32_t held[kAhead][kWordColumns];
     uint32_t all = 0, mine = 0, ahead_tile = pair, ahead_stage = 0;
     for (uint32_t tile = pair; tile < tiles; tile += pairs) all += k_stages;
     Place ahead = {};
     if (all > 0) ahead = place(pair);
     // Nothing looks at them before they are laid down, so that nothing waits for them here.
-    auto fetch = [&](uint32_t (&into)[kWords]) {
+    auto fetch = [&](uint32_t (&into)[kWordColumns]) {
       if (mine >= all) return;
       ++mine;
-      const uint32_t at = ahead_stage * kStageWords + group;
-      const uint32_t* const source = of_x ? p.x_scales + (size_t)at * p.m : p.w_scales + (size_t)at * p.w_rows;
-      const uint32_t first = of_x ? ahead.row : ahead.w_row + rank * kColumns, end = at >= words ? 0u : of_x ? ahead.end : min(p.w_rows, first + kColumns);
+      const uint32_t at = ahead_stage * kStageWords + group, w_row = ahead.w_row + rank * kColumns + lane, x_row = ahead.row + lane;
+      const uint32_t w_end = at < words ? p.w_rows : 0u, x_end = at < words ? ahead.end : 0u;
+      const uint32_t *const of_w = p.w_scales + (size_t)at * p.w_rows, *const of_x = p.x_scales + (size_t)at * p.m;
 #pragma unroll
-      for (uint32_t i = 0; i < kWords; ++i) {
+      for (uint32_t i = 0; i < 4; ++i) {
         into[i] = 0u;
-        if (first + i * 32u + lane < end) into[i] = source[first + i * 32u + lane];
+        if (w_row + i * 32u < w_end) into[i] = of_w[w_row + i * 32u];
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < 4 * kInputAtoms; ++i) {
+        into[4 + i] = 0u;
+        if (x_row + i * 32u < x_end) into[4 + i] = of_x[x_row + i * 32u];
       }
       if (++ahead_stage == k_stages) {
         ahead_stage = 0;
@@ -251,23 +258,27 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint32_t mask = ks * kStageWords + group + 1u == words ? last_mask : 0xffffffffu;
-        const uint32_t(&v)[kWords] = held[a];
-        unsigned char* const line = base_pointer + s * kStageBytes + (of_x ? kInputScalesAt + group * kInputAtoms * kAtom : kScalesAt + group * kAtom) + lane * 16u;
-        *reinterpret_cast<uint4*>(line) = make_uint4(v[0] & mask, v[1] & mask, v[2] & mask, v[3] & mask);
-        if (of_x) *reinterpret_cast<uint4*>(line + kAtom) = make_uint4(v[4] & mask, v[5] & mask, v[6] & mask, v[7] & mask);
+        const uint32_t(&v)[kWordColumns] = held[a];
+        unsigned char* const stage = base_pointer + work.ring + s * work.stage_bytes;
+        auto line = [&](uint32_t atom, uint32_t first) {  // a lane's four rows are a line of an atom
+          *reinterpret_cast<uint4*>(stage + atom + lane * 16u) = make_uint4(v[first] & mask, v[first + 1] & mask, v[first + 2] & mask, v[first + 3] & mask);
+        };
+        line(kScalesAt + group * kAtom, 0u);
+        line(kInputScalesAt + group * kInputAtoms * kAtom, 4u);
+        line(kInputScalesAt + (group * kInputAtoms + 1u) * kAtom, 8u);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) first_arrive(first_address(scales_full + s * 8));
         fetch(held[a]);
         if (++ks == k_stages) ks = 0;
-        if (++s == kStages) s = 0, phase ^= 1u;
+        if (++s == work.stages) s = 0, phase ^= 1u;
       }
     }
     if (!ok) give_up();
   } else {
     const uint32_t worker = warp - 2u - kScaleWarps, quarter = warp & 3u, side = worker >> 2;  // lanes of tensor memory; every other piece
-    unsigned char* const staging = base_pointer + kStaging + worker * kWarpStaging;
-    uint32_t turn = 0, turn_of_box = 0;
+    unsigned char* const staging = base_pointer + kFront + worker * kStagingBytes;
+    uint32_t turn = 0;
     bool ok = true;
     for (uint32_t tile = pair; tile < tiles && ok; tile += pairs, ++turn) {
       const uint32_t which = turn % kSums;
@@ -289,19 +300,14 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         constexpr uint32_t kWidth = kPaired<S> ? 16 : 32;  // columns of results
         const uint32_t out_column = kPaired<S> ? column / 2u : column, columns = kPaired<S> ? p.n / 2u : p.n;
+        if (lane == 0) await_box();
+        __syncwarp();
         if (S != kStoreFloat && work.boxes && row + 32u <= at.end && out_column + kWidth <= columns) {
-          // whole pieces: one of two boxes is filled while the other is on its way
-          unsigned char* const box = staging + turn_of_box * kBoxBytes;
-          if (lane == 0) await_boxes<1>();
-          __syncwarp();
-          if constexpr (S != kStoreFloat) stage_piece<S, kWidth * 2>(p, row, at.end, column, raw, box);
+          if constexpr (S != kStoreFloat) stage_piece<S, kWidth * 2>(p, row, at.end, column, raw, staging);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0) store_box(&map_out, (int32_t)out_column, (int32_t)row, smem_u32(box));
-          turn_of_box ^= 1u;
+          if (lane == 0) store_box(&map_out, (int32_t)out_column, (int32_t)row, smem_u32(staging));
         } else {
-          if (lane == 0) await_boxes<0>();
-          __syncwarp();
           store_piece<S>(p, row, at.end, column, raw, staging);
         }
         __syncwarp();  // tcgen05.ld needs the whole warp
@@ -310,7 +316,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       __syncwarp();
       if (lane == 0) first_arrive(first_address(sums_empty + which * 8));
     }
-    if (lane == 0) await_boxes<0>();
+    if (lane == 0) await_box();
     __syncwarp();
   }
 
@@ -329,22 +335,25 @@ namespace mxfp4 {
 template <Store S>
 int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
   const uint32_t pairs = (uint32_t)context_sm_count(args.ctx) / 2u, k_stages = (p.k + kDepth - 1u) / kDepth;
-  Work work = {plan_tiles, (p.n + 2u * kColumns - 1u) / (2u * kColumns), kExpertTile, 16u, 0u};
+  Work work = {plan_tiles, (p.n + 2u * kColumns - 1u) / (2u * kColumns), kExpertTile, 0u, 0u, 0u, 0u};
   if (!p.plan.tiles) {
-    // the height with the shortest estimate: rounds of tiles times the cycles of one, of which a stage takes about 280 and one per row
+    // the height with the shortest estimate: rounds of tiles times the cycles of one, of which a stage takes about 500 and four per row
     uint64_t least = ~0ull;
     for (uint32_t rows = kLoneRows; rows >= 32u; rows -= 32u) {
       const uint32_t row_tiles = (p.m + rows - 1u) / rows;
       if (rows > kMostRows && (uint64_t)row_tiles * work.column_tiles > pairs) continue;  // its sums lie over those of the next
-      const uint64_t rounds = ((uint64_t)row_tiles * work.column_tiles + pairs - 1u) / pairs, cost = rounds * ((uint64_t)k_stages * (280u + rows) + 1000u);
+      const uint64_t rounds = ((uint64_t)row_tiles * work.column_tiles + pairs - 1u) / pairs, cost = rounds * ((uint64_t)k_stages * (500u + 4u * rows) + 1000u);
       if (cost < least) least = cost, work.rows = rows, work.row_tiles = row_tiles;
     }
-    work.box_rows = work.rows / 2u;
   }
   const uint64_t tiles = (uint64_t)work.row_tiles * work.column_tiles;
   LLMOPT_REQUIRE(tiles < (1u << 28), "too many tiles");
+  work.stage_bytes = kInputAt + kBoxes * (work.rows / 2u * kRowBytes);
+  work.ring = kFront + (tiles > pairs ? kStaging : 0u);
+  work.stages = (kMostShared - 1024u - work.ring) / work.stage_bytes;
+  if (work.stages > kMostStages) work.stages = kMostStages;
   CUtensorMap map_w, map_x;
-  LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.box_rows), "tensor map was refused");
+  LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.rows / 2u), "tensor map was refused");
   CUtensorMap map_out = map_x;  // not read without boxes
   const uint32_t columns = kPaired<S> ? p.n / 2u : p.n;
   if (S != kStoreFloat && columns % 8u == 0 && ((uintptr_t)p.out & 15u) == 0) {
@@ -352,8 +361,8 @@ int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
     work.boxes = make_map(&map_out, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2u, p.out, columns, p.m,
                           kPaired<S> ? 16u : 32u, 32u, CU_TENSOR_MAP_SWIZZLE_NONE);
   }
-  LLMOPT_REQUIRE(allow_shared(tiles_kernel<S>, kSharedBytes), "shared memory request was refused");
-  launch_cluster_kernel(args, tiles_kernel<S>, dim3(2u * (tiles < pairs ? (uint32_t)tiles : pairs)), dim3(kThreads), kSharedBytes, 2u, map_w, map_x, map_out, p,
+  LLMOPT_REQUIRE(allow_shared(tiles_kernel<S>, kMostShared), "shared memory request was refused");
+  launch_cluster_kernel(args, tiles_kernel<S>, dim3(2u * (tiles < pairs ? (uint32_t)tiles : pairs)), dim3(kThreads), 1024u + work.ring + work.stages * work.stage_bytes, 2u, map_w, map_x, map_out, p,
                         work, context_device_error(args.ctx));
   return check_launch(args);
 }
