@@ -23,9 +23,14 @@ int check_operands(const KernelArgs& args, const Problem& p) {
 template <Store S>
 int run_product(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
   LLMOPT_REQUIRE(args.ctx != nullptr, "needs a context");
-  // us, stream and tiles: 64 rows through 4096 x 14336 10.2, 12.4, through 4096 x 128256 56, 57; sorted rows through 4096 x 7168 of 16 experts,
-  // 64 of them 36.7, 38.5, 256 44, 42, 1024 66, 53
-  return p.m <= 64u ? run_stream<S>(args, p, plan_tiles) : run_tiles<S>(args, p, plan_tiles);
+  // Up to 64 rows the stream, us beside the tiles': 64 rows through 4096 x 14336 10.4, 12.2, k 14336 x 4096 12.7, 18.4; 32 sorted rows of 16 experts
+  // through 4096 x 7168 25.7, 28.2.  Tiles that would be more than 13 CTAs for every two SMs go to the kernel whose CTAs stay for the next
+  // (stream, tiles: 448 tiles, 32 rows through 4096 x 57344 26.7, 28.7; 896, 64 sorted rows through 4096 x 7168 37.2, 36.7; 1002, 4096 x 128256
+  // 32 rows 53.6, 51.8, 64 rows 58.3, 54.4; 1024, 64 sorted rows of 64 experts 15.6, 14.8; 7168, 64 of 128 experts 110, 80), unless all read the
+  // same rows and those are few (1 row through 4096 x 128256 48.8, 50.0, 16 rows 51.6, 51.1).
+  const uint64_t tiles = (uint64_t)(p.plan.tiles ? plan_tiles : 1u) * ((p.n + kColumns - 1u) / kColumns);
+  const bool few = tiles * 2u <= (uint64_t)context_sm_count(args.ctx) * 13u || (!p.plan.tiles && p.m <= 16u);
+  return p.m <= 64u && few ? run_stream<S>(args, p, plan_tiles) : run_tiles<S>(args, p, plan_tiles);
 }
 
 Problem operands(const KernelArgs& args) {

@@ -220,7 +220,7 @@ def test_one_block_at_a_time_meets_its_exponents(runtime):
 
 # rows and columns in other numbers than the tiles have, one to several tiles for every pair of SMs, sums shared out over a cluster's CTAs
 SIZES = [(48, 8192, 8192), (17, 4096, 4096), (64, 4096, 14336), (1, 128256, 256), (33, 20000, 512), (65, 9472, 512), (224, 18944, 256), (225, 2560, 1024),
-         (256, 14336, 512), (448, 4736, 288), (777, 7168, 256), (1000, 1000, 1000 // 32 * 32), (3000, 600, 128), (90, 40, 16384)]
+         (256, 14336, 512), (448, 4736, 288), (777, 7168, 256), (1000, 1000, 1000 // 32 * 32), (3000, 600, 128), (90, 40, 16384), (16, 123400, 160), (17, 123400, 160), (64, 128256, 256)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -307,7 +307,8 @@ def expert_case(rng, counts, n, k):
 
 
 EXPERTS = [([1], 2, 32), ([0, 0, 1], 64, 160), ([1, 1], 7168, 1024), ([3, 0, 1, 0, 0, 2, 1, 1], 258, 576), ([0, 5, 11, 0], 130, 2048),
-           ([128, 127, 129, 0, 1], 96, 416), ([300], 200, 256), ([0, 700, 3, 0, 65], 320, 1792), ([2] * 40, 32, 96), ([17, 33, 64, 40], 500, 736)]
+           ([128, 127, 129, 0, 1], 96, 416), ([300], 200, 256), ([0, 700, 3, 0, 65], 320, 1792), ([2] * 40, 32, 96), ([17, 33, 64, 40], 500, 736),
+           ([1, 3] * 12, 5400, 96), ([40, 0, 1] + [1] * 19, 6000, 544)]
 
 
 @pytest.mark.parametrize("case", range(len(EXPERTS)))
