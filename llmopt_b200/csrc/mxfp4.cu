@@ -13,6 +13,8 @@ namespace llmopt {
 namespace {
 using namespace mxfp4;
 
+// Both are bound by HBM, few rows by the launch: values of 14336 x 4096 fp32 into codes 45 us, 5.7 TB/s, and back 45 to 49, 5.1 to 5.7;
+// 4096 rows gathered from 2048 x 4096 bf16 10.0; 1 x 4096 2.6.  All of a CTA's values are asked for before the first is looked at.
 // A CTA takes 32 rows x 256 columns, a warp four of the rows, 16 bytes of values per lane and access: 256 columns of 16 bits at a
 // time, 128 of 32.  The exponents of the 32 rows leave together, 128 bytes of a word's row.
 constexpr uint32_t kTileRows = 32, kTileColumns = 256, kWarps = 8, kRowsPerWarp = kTileRows / kWarps;
@@ -83,8 +85,9 @@ __device__ __forceinline__ uint32_t load_codes(const uint8_t* source) {
 }
 
 template <typename T, bool GATHER>
-__global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 4 ? 5 : 6) quantize_kernel(const T* x, const uint32_t* index, uint8_t* codes, uint32_t* scales, uint32_t rows,
-                                                               uint32_t source_rows, uint32_t k, size_t stride, bool vectors) {
+__global__ void __launch_bounds__(kWarps * 32, sizeof(T) == 4 ? 5 : 6)
+quantize_kernel(const T* x, const uint32_t* index, uint8_t* codes, uint32_t* scales, uint32_t rows, uint32_t source_rows, uint32_t k, size_t stride,
+                bool vectors) {
   using A = Access<T>;
   grid_chain_prologue();
   __shared__ uint32_t words[2][kTileRows];

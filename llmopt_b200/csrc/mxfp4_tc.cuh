@@ -17,10 +17,10 @@ uint32_t* context_device_error(Context* ctx);
 namespace mxfp4 {
 using namespace tc;
 
-constexpr uint32_t kColumns = 128;                                        // weight rows of a tile
-constexpr uint32_t kBoxDepth = 256, kRowBytes = kBoxDepth / 2;            // elements of k of a box of codes
-constexpr uint32_t kAtom = 512;                                           // an atom: the words of 128 rows
-constexpr uint32_t kScaleWarps = 4;  // a thread per weight row
+constexpr uint32_t kColumns = 128;                              // weight rows of a tile
+constexpr uint32_t kBoxDepth = 256, kRowBytes = kBoxDepth / 2;  // elements of k of a box of codes
+constexpr uint32_t kAtom = 512;                                 // an atom: the words of 128 rows
+constexpr uint32_t kScaleWarps = 4;                             // a warp per word of a stage
 
 // One lane of a converged warp.  What the tensor cores and copies take lies in uniform registers: where the whole warp walks through a loop
 // with values that are the same in all lanes and one lane issues, they are kept there; a loop that one lane walks through alone
@@ -66,8 +66,8 @@ template <> struct Element<kStorePairBf16> { typedef bf16 Type; };
 __device__ __forceinline__ uint32_t packed(__half a, __half b) { return (uint32_t)__half_as_ushort(a) | (uint32_t)__half_as_ushort(b) << 16; }
 __device__ __forceinline__ uint32_t packed(bf16 a, bf16 b) { return (uint32_t)__bfloat16_as_ushort(a) | (uint32_t)__bfloat16_as_ushort(b) << 16; }
 
-// silu whose exponential and quotient are off by two steps of fp32 each, and by one of the exponent: of a result in sixteen bits that is
-// nothing, and with the exact quotient the pairs of a tile took longer than its products (9.0 against 5.2 us).
+// silu whose exponential and quotient are off by a few steps of fp32 (and below -87, where it is under 2^-118, by all of it): of a result
+// in sixteen bits that is nothing, and with the exact quotient the pairs of a tile took longer than its products (9.0 against 5.2 us).
 __device__ __forceinline__ float silu_short(float z) { return __fdividef(z, 1.0f + __expf(-z)); }
 
 // Sums of COUNT rows from `row` on, of the output column that is this lane's, on their way out; the whole warp takes part.  Sixteen-bit

@@ -1,13 +1,21 @@
 // Products of many MXFP4 rows: pairs of CTAs walk over tiles of 256 weight rows by up to 224 rows of x (256 where no pair has a second tile).
 //
-// What bounds a tile is how often its operands come from L2: tcgen05.mma with cta_group::2 multiplies 256 weight rows, half of them in
-// either CTA's shared memory, with rows of x of which either CTA holds half as well, 30 KB for what a CTA by itself needs 44 KB for.
-// In each CTA warp 0 brings the codes of 256 elements of k of its halves by TMA (128-byte swizzle); warps 2 and 3 bring the exponents of
-// its 128 weight rows, warps 4 and 5 those of all rows of x, a warp per word of a stage, requested four stages ahead and laid down
-// in the order that tcgen05.cp spreads over tensor memory.  One lane of warp 1 of the first CTA issues copies and products for
-// both, and its barriers count both CTAs' copies and exponents.  Eight more warps read a tile's sums out, each a quarter of the
-// lanes (output columns), while the next tile's are formed in other columns of tensor memory; results of 16 bits change
-// places in shared memory, so that four lanes share 64 bytes of a row.
+// Why pairs: a tile's operands come from L2, and tcgen05.mma with cta_group::2 multiplies 256 weight rows, half of them in either
+// CTA's shared memory, with rows of x of which either CTA holds half as well: per 256 elements of k 30 KB a CTA where one by itself needs
+// 44 KB.  In each CTA warp 0 brings the codes of 512 elements of k of its halves by TMA (128-byte swizzle); warps 2 to 5 bring
+// exponents, a warp per word of a stage, those of the CTA's 128 weight rows and of all rows of x, requested three stages ahead and laid
+// down in the order that tcgen05.cp spreads over tensor memory.  One lane of warp 1 of the first CTA issues copies and products
+// for both, and its barriers count both CTAs' copies and exponents.  Eight more warps read a tile's sums out, each a quarter of the lanes
+// (output columns), while the next tile's are formed in other columns of tensor memory; results of 16 bits change places in shared
+// memory and leave as boxes of 32 rows by TMA, ragged ones by vector stores.
+//
+// What bounds it: a stage costs the tensor cores 4 cycles per row of x, about 50 per copy of exponents (they share the pipe: 12 of them)
+// and a handover of the ring, together close to 500 + 4 rows.  Stages of 512 rather than 256 elements halve the handovers: 4096 x
+// 4096 x 14336 108 -> 99 us, 2048 x 4096 x 4096 24.9 -> 21.3, 512 x 14336 x 4096 25.7 -> 20.9.  The large product then runs at 4.86
+// PFLOP/s, and k 8192 at 5.45; repeated for a second it draws the part's 1000 W and takes 111 us at 1.6 to 1.7 GHz.  Rows sorted by expert
+// have tiles of 128, which spend half a stage outside the products: 4096 of 16 experts through 4096 x 7168 88 us, 2.7 PFLOP/s and 2.9
+// TB/s.  Joined into tiles of up to 224 they took 87, but rows of 64 experts 116 where these take 106: taller boxes leave three stages for
+// four.
 //
 // Every wait on an mbarrier is bounded; a wait that runs out raises the context's device error word, and the CTA lets its copies and
 // products end, frees its tensor memory and returns.
@@ -27,7 +35,7 @@ constexpr uint32_t kBoxBytes = kColumns * kRowBytes;  // of weights
 // stages there are.
 constexpr uint32_t kScalesAt = kBoxes * kBoxBytes, kInputScalesAt = kScalesAt + kStageWords * kAtom;
 constexpr uint32_t kInputAt = kInputScalesAt + kStageWords * kInputAtoms * kAtom;
-constexpr uint32_t kMostStages = 4, kSums = 2;
+constexpr uint32_t kMostStages = 4, kSums = 2;  // sums of two tiles in tensor memory
 constexpr uint32_t kWordColumns = 4 * (1 + kInputAtoms), kScaleColumns = kStageWords * kWordColumns, kTmemColumns = 512;
 static_assert(kSums * kMostRows + kScaleColumns <= kTmemColumns && kInputAt % 1024 == 0, "tensor memory, alignment of tiles");
 // In front of the ring: barriers, tensor memory's address, abort flag, and the staging of the warps that store, which lies over the ring where
@@ -38,10 +46,10 @@ static_assert(kAbort + 4 <= kFront && kStaging % 1024 == 0, "alignment of tiles"
 static_assert(kStagingBytes >= 32 * 64, "a box of results");
 
 struct Work {
-  uint32_t row_tiles, column_tiles;  // of x, of pairs of weight tiles
-  uint32_t rows;                     // most of a tile; either CTA copies half of them, whatever there are
-  uint32_t stages, stage_bytes, ring;
-  uint32_t boxes;                    // results leave in boxes
+  uint32_t row_tiles, column_tiles;    // of x, of pairs of weight tiles
+  uint32_t rows;                       // most of a tile; either CTA copies half of them, whatever there are
+  uint32_t stages, stage_bytes, ring;  // of shared memory; where the ring begins
+  uint32_t boxes;                      // results leave in boxes
 };
 
 // The first CTA's barriers, from either.
@@ -362,8 +370,9 @@ int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
                           kPaired<S> ? 16u : 32u, 32u, CU_TENSOR_MAP_SWIZZLE_NONE);
   }
   LLMOPT_REQUIRE(allow_shared(tiles_kernel<S>, kMostShared), "shared memory request was refused");
-  launch_cluster_kernel(args, tiles_kernel<S>, dim3(2u * (tiles < pairs ? (uint32_t)tiles : pairs)), dim3(kThreads), 1024u + work.ring + work.stages * work.stage_bytes, 2u, map_w, map_x, map_out, p,
-                        work, context_device_error(args.ctx));
+  const uint32_t shared = 1024u + work.ring + work.stages * work.stage_bytes;  // 1024 for the alignment of the ring
+  launch_cluster_kernel(args, tiles_kernel<S>, dim3(2u * (tiles < pairs ? (uint32_t)tiles : pairs)), dim3(kThreads), shared, 2u, map_w, map_x,
+                        map_out, p, work, context_device_error(args.ctx));
   return check_launch(args);
 }
 

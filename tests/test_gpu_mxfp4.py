@@ -308,7 +308,8 @@ def expert_case(rng, counts, n, k):
 
 EXPERTS = [([1], 2, 32), ([0, 0, 1], 64, 160), ([1, 1], 7168, 1024), ([3, 0, 1, 0, 0, 2, 1, 1], 258, 576), ([0, 5, 11, 0], 130, 2048),
            ([128, 127, 129, 0, 1], 96, 416), ([300], 200, 256), ([0, 700, 3, 0, 65], 320, 1792), ([2] * 40, 32, 96), ([17, 33, 64, 40], 500, 736),
-           ([1, 3] * 12, 5400, 96), ([40, 0, 1] + [1] * 19, 6000, 544)]
+           ([1, 3] * 12, 5400, 96), ([40, 0, 1] + [1] * 19, 6000, 544),
+           ([225, 224, 449, 1, 128], 322, 352), ([5000, 40, 0, 3000], 64, 64), ([1, 0, 400], 4736, 1056)]
 
 
 @pytest.mark.parametrize("case", range(len(EXPERTS)))
@@ -371,6 +372,32 @@ def test_expert_rows_without_a_tile_stay_as_they_were(runtime):
     dispatch.dispatch_mxfp4_expert_rows(context(runtime), **operands, plan=device(runtime, plan).buffer, output=y)
     got = read(y, 256)
     assert np.allclose(got[6:], xv[6:] @ wv[n:].T, rtol=1e-5, atol=1e-3)
+
+
+def test_many_expert_rows_follow_the_plan(runtime):
+    """Rows between the tiles stay as they were, and what points outside is cut."""
+    from llmopt_b200 import dispatch
+
+    rng = np.random.default_rng(13)
+    n, k, slots = 96, 256, 600
+    x, w = random_operand(rng, slots, k), random_operand(rng, 2 * n, k)
+    xt, wt = upload(runtime, x), upload(runtime, w)
+    plan = np.zeros((1 + slots // 128 + 2, 4), np.uint32)
+    plan[0, 0] = 1000  # more tiles than it has room for; an end and an expert that are not there; tiles without rows
+    plan[1:5] = (0, 0, 128, 0), (0, 128, 5000, 0), (0, 270, 300, 0), (7, 590, 2 ** 32 - 1, 0)
+    y = blank(runtime, (slots, n), "float32", 256)
+    dispatch.dispatch_mxfp4_expert_rows(context(runtime), input=xt[0], input_scales=xt[1], weight=wt[0], weight_scales=wt[1], experts=2,
+                                        plan=device(runtime, plan).buffer, output=y)
+    got = read(y, 256)
+    untouched = np.full(4, CANARY, np.uint8).view(np.float32)[0]
+    expert = np.full(slots, -1)
+    expert[:256], expert[270:300], expert[590:] = 0, 0, 1
+    xv, wv = mx.values(*x), mx.values(*w)
+    assert (got[expert < 0] == untouched).all()
+    for e in (0, 1):
+        mine = wv[e * n:(e + 1) * n]
+        want = xv[expert == e] @ mine.T
+        check(got[expert == e].astype(np.float64), want, allowed(xv[expert == e], mine, want, "float32"))
 
 
 # ---- as they are used -------------------------------------------------------------------------------------
