@@ -317,10 +317,10 @@ int run(const KernelArgs& args, const Problem& p, uint32_t row_tiles) {
   const uint32_t rows = p.m < NT ? p.m : NT;
   work.share = (rows + work.splits - 1u) / work.splits;
   while (shared_bytes<NT>(work) > kMostShared) --work.stages;
-  CUtensorMap map_w, map_x;
-  LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.box_rows), "tensor map was refused");
   auto kernel = stream_kernel<NT, S>;
   LLMOPT_REQUIRE(allow_shared(kernel, kMostShared), "shared memory request was refused");
+  CUtensorMap map_w, map_x;
+  LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.box_rows), "tensor map was refused");
   const dim3 grid((uint32_t)tiles * work.splits);
   if (work.splits == 1u)
     launch_kernel(args, kernel, grid, dim3(kThreads), shared_bytes<NT>(work), map_w, map_x, p, work, context_device_error(args.ctx));

@@ -221,7 +221,8 @@ inline bool make_map(CUtensorMap* map, const void* codes, uint64_t k, uint64_t r
   return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1u, codes, k / 2, rows, kRowBytes, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Lets a kernel have as much shared memory as any launch of it asks for: the limit is one per kernel, whoever launches it.
+// Lets a kernel have as much shared memory as any launch of it asks for: the limit is one per kernel, whoever launches it.  Ahead of make_map, whose call
+// does not give a thread its context as this one does.
 template <typename... Params>
 bool allow_shared(void (*kernel)(Params...), uint32_t bytes) {
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess) return true;

@@ -171,6 +171,9 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     if (rank == 0u && (!ok || *abort_flag))
       for (uint32_t i = issued > work.stages ? issued - work.stages : 0u; i < issued; ++i)
         barrier_wait(full + (i % work.stages) * 8, (i / work.stages) & 1u);
+    // but for a stage that only the second one came to ask for, which nothing counts any more: it has a millisecond to land
+    if (rank == 1u && (!ok || *abort_flag))
+      for (uint32_t i = 0; i < 1000u; ++i) __nanosleep(1000);
     __syncwarp();
   } else if (warp == 1 && rank == 1u) {
     // the first CTA issues for both
@@ -360,6 +363,7 @@ int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
   work.ring = kFront + (tiles > pairs ? kStaging : 0u);
   work.stages = (kMostShared - 1024u - work.ring) / work.stage_bytes;
   if (work.stages > kMostStages) work.stages = kMostStages;
+  LLMOPT_REQUIRE(allow_shared(tiles_kernel<S>, kMostShared), "shared memory request was refused");
   CUtensorMap map_w, map_x;
   LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.rows / 2u), "tensor map was refused");
   CUtensorMap map_out = map_x;  // not read without boxes
@@ -369,7 +373,6 @@ int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
     work.boxes = make_map(&map_out, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2u, p.out, columns, p.m,
                           kPaired<S> ? 16u : 32u, 32u, CU_TENSOR_MAP_SWIZZLE_NONE);
   }
-  LLMOPT_REQUIRE(allow_shared(tiles_kernel<S>, kMostShared), "shared memory request was refused");
   const uint32_t shared = 1024u + work.ring + work.stages * work.stage_bytes;  // 1024 for the alignment of the ring
   launch_cluster_kernel(args, tiles_kernel<S>, dim3(2u * (tiles < pairs ? (uint32_t)tiles : pairs)), dim3(kThreads), shared, 2u, map_w, map_x,
                         map_out, p, work, context_device_error(args.ctx));

@@ -351,6 +351,11 @@ def _mxfp4_operand_ok(codes: Tensor, scales: Tensor, rows: int, k: int) -> bool:
             and tuple(scales.shape) == (mxfp4_scale_words(k), rows))
 
 
+def _mxfp4_rows(*tensors: Tensor) -> None:
+    if any(len(tensor.shape) != 2 for tensor in tensors):
+        raise DispatchError("MXFP4 operands must have rank two")
+
+
 def _mxfp4_element(tensor: Tensor, most: str) -> str:
     element = _MXFP4_ELEMENTS.get(tensor.dtype)
     if element is None or (most == "16" and element == "f32"):
@@ -363,8 +368,7 @@ def dispatch_mxfp4_quantize(context: Context, *, input: Tensor, codes: Tensor, s
     """Rows of ``input`` [rows, stride] (their first ``columns``, all if None) to ``codes`` u8 [slots, k / 2] and ``scales`` u32
     [ceil(k / 128), slots]; with ``row_of_slot`` u32 [slots] the rows that it names, as routed experts read them."""
     element = _mxfp4_element(input, "32")
-    if len(input.shape) != 2:
-        raise DispatchError("MXFP4 quantization input must have rank two")
+    _mxfp4_rows(input)
     source_rows, stride = input.shape
     k = stride if columns is None else columns
     slots = source_rows if row_of_slot is None else row_of_slot.numel
@@ -392,6 +396,7 @@ def dispatch_mxfp4_dequantize(context: Context, *, codes: Tensor, scales: Tensor
 def dispatch_mxfp4_linear(context: Context, *, input: Tensor, input_scales: Tensor, weight: Tensor, weight_scales: Tensor,
                           output: Tensor, bias: Optional[Tensor] = None) -> list:
     """``output`` [m, n] = ``input`` [m, k] . ``weight`` [n, k]^T (+ ``bias`` [n], in the output's type), both in MXFP4, sums in fp32."""
+    _mxfp4_rows(input, weight)
     element = _mxfp4_element(output, "32")
     m, n, k = input.shape[0], weight.shape[0], 2 * weight.shape[1]
     if k % 32 != 0 or not (_mxfp4_operand_ok(input, input_scales, m, k) and _mxfp4_operand_ok(weight, weight_scales, n, k)):
@@ -409,6 +414,7 @@ def dispatch_mxfp4_expert_rows(context: Context, *, input: Tensor, input_scales:
     """Rows sorted by expert (``plan`` of ``llmopt_route_plan``) times their experts' matrices, ``weight`` [experts * n, k / 2].  With
     ``score_of_slot`` f32 [slots] neighbouring columns are a gate and a value and ``output`` [slots, n / 2], f16 or bf16, is
     silu(score * gate) * (score * value); without, it is f32 [slots, n]."""
+    _mxfp4_rows(input, weight)
     paired = score_of_slot is not None
     slots, k = input.shape[0], 2 * weight.shape[1]
     if experts <= 0 or weight.shape[0] % experts != 0 or (paired and weight.shape[0] // experts % 2 != 0):

@@ -649,6 +649,43 @@ def test_pointers_streams_and_captured_calls(runtime):
             checked(c, x)
 
 
+def test_calls_from_several_threads(runtime):
+    """Streams with clusters and pairs of CTAs side by side, each from a thread of its own: whole numbers, which come out exactly."""
+    import threading
+
+    import torch
+
+    torch.cuda.init()
+    rng = np.random.default_rng(31)
+    pick = np.array([0, 2, 4, 5, 10, 12, 13], np.uint8)
+    cases = []
+    for m, n, k in ((3, 4096, 4096), (64, 2048, 8192), (300, 2304, 2048), (129, 9472, 512)):
+        x, w = rng.choice(pick, (m, k)), rng.choice(pick, (n, k))
+        ones = [np.full((rows, k // 32), 127, np.uint8) for rows in (m, n)]
+        want = torch.from_numpy((mx.values(x, ones[0]).astype(np.float32) @ mx.values(w, ones[1]).astype(np.float32).T)).cuda()
+        operands = [torch.from_numpy(a).cuda() for a in (mx.pack(x), mx.words(ones[0]).view(np.int32), mx.pack(w), mx.words(ones[1]).view(np.int32))]
+        cases.append((m, n, k, operands, [torch.empty(m, n, device="cuda") for _ in range(20)], want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    failed = []
+
+    def run(m, n, k, operands, results, want, stream):
+        try:
+            for y in results:
+                runtime.mxfp4_linear_pointers("f32", *[t.data_ptr() for t in operands], None, y.data_ptr(), m, n, k, stream.cuda_stream)
+        except Exception as error:
+            failed.append(error)
+
+    threads = [threading.Thread(target=run, args=case) for case in cases]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for _, _, _, _, results, want, _ in cases:
+        assert all(torch.equal(y, want) for y in results)
+
+
 def test_expert_rows_of_pointers(runtime):
     import torch
 

@@ -103,13 +103,13 @@ def test_dispatchers_refuse_inconsistent_operands():
     for wrong in (dict(input=_tensor("c", (5, 32), "uint8")), dict(input=_tensor("c", (5, 48), "int8")),
                   dict(input_scales=_tensor("s", (5, 1), "uint32")), dict(weight_scales=_tensor("ws", (2, 12), "uint32")),
                   dict(weight=_tensor("w", (12, 40), "uint8")), dict(output=_tensor("y", (5, 11), "float16")),
-                  dict(output=_tensor("y", (5, 12), "float64")), dict(bias=_tensor("b", (12,), "float32")),
+                  dict(weight=_tensor("w", (576,), "uint8")), dict(input=_tensor("c", (), "uint8")), dict(output=_tensor("y", (5, 12), "float64")), dict(bias=_tensor("b", (12,), "float32")),
                   dict(bias=_tensor("b", (11,), "float16"))):
         with pytest.raises(dispatch.DispatchError):
             dispatch.dispatch_mxfp4_linear(context, **{**good, "output": y, **wrong})
     score = _tensor("g", (5,), "float32")
     experts = dict(**good, experts=3, plan="plan", output=_tensor("y", (5, 2), "bfloat16"), score_of_slot=score)
-    for wrong in (dict(experts=5), dict(experts=4), dict(experts=0), dict(output=_tensor("y", (5, 2), "float32")),
+    for wrong in (dict(experts=5), dict(experts=4), dict(experts=0), dict(weight=_tensor("w", (576,), "uint8")), dict(output=_tensor("y", (5, 2), "float32")),
                   dict(output=_tensor("y", (5, 4), "bfloat16")), dict(score_of_slot=None), dict(score_of_slot=_tensor("g", (4,), "float32"))):
         with pytest.raises(dispatch.DispatchError):
             dispatch.dispatch_mxfp4_expert_rows(context, **{**experts, **wrong})
