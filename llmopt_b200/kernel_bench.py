@@ -4,7 +4,7 @@ as achieved GB/s over the algorithmic bytes.  The counterpart of the reference's
 stand-alone Metal tile probes (bench/metal_q4_tile_probe.swift); also the small,
 self-terminating command used for profiler captures.
 
-  python -m llmopt_b200.kernel_bench --op linear|linear_affine|qkv|gate_up|down|lm_head|attention|q4_0|dense_attention \\
+  python -m llmopt_b200.kernel_bench --op linear|linear_affine|qkv|gate_up|down|lm_head|attention|q4_0|mxfp4|dense_attention \\
          --m 1 --k 4096 --n 14336 [--heads 32 --kv-heads 8 --dim 128 --past 8192] [--iters 20]
 """
 
@@ -122,6 +122,15 @@ def build_item(runtime, args):
             weight=dispatch.Tensor(Buffer.of_array(runtime, blocks), (n, (k // 32) * 18), "uint8"),
             output=_f16(runtime, rng, (m, n)))
         nbytes = n * (k // 32) * 18 + m * k * 2 + m * n * 2
+    elif args.op == "mxfp4":
+        def operand(rows):
+            words = dispatch.mxfp4_scale_words(k)
+            return (dispatch.Tensor(Buffer.of_array(runtime, rng.integers(0, 256, (rows, k // 2), dtype=np.uint8)), (rows, k // 2), "uint8"),
+                    dispatch.Tensor(Buffer.of_array(runtime, rng.integers(120, 134, (words, rows, 4), dtype=np.uint8)), (words, rows), "uint32"))
+        (x, x_scales), (w, w_scales) = operand(m), operand(n)
+        dispatch.dispatch_mxfp4_linear(context, input=x, input_scales=x_scales, weight=w, weight_scales=w_scales,
+                                       output=_f16(runtime, rng, (m, n)))
+        nbytes = (m + n) * (k // 2 + k // 32) + m * n * 2
     elif args.op == "dense_attention":
         # causal prefill attention over m query = key rows: query / key head-major, value and output token-first
         tokens = m
