@@ -236,6 +236,8 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         if (++s == work.stages) s = 0, phase ^= 1u;
       }
     }
+    const uint32_t quarter = warp & 3u;
+    float own = splits == 1u ? piece_operand<S>(p, at.row, at.end, at.column + quarter * 32u) : 0.0f;
     if (ok) {
       ok = !*abort_flag && warp_wait(sums_full, 0u);
       ok = __all_sync(0xffffffffu, ok);
@@ -245,7 +247,7 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
       give_up();
     } else {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t quarter = warp & 3u, address = tmem_base + ((quarter * 32u) << 16), place = quarter * 32u + lane;
+      const uint32_t address = tmem_base + ((quarter * 32u) << 16), place = quarter * 32u + lane;
       uint32_t owner = 0, share_row = 0;
 #pragma unroll 1
       for (uint32_t piece = 0; piece < NT / Z::kPiece; ++piece) {
@@ -257,7 +259,8 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         if (splits == 1u) {
           // through the ring: every stage of it has been read
-          store_piece<S>(p, row, at.end, at.column + quarter * 32u, raw, base_pointer + quarter * kStagingBytes);
+          if (kPaired<S> && piece > 0) own = piece_operand<S>(p, row, at.end, at.column + quarter * 32u);
+          store_piece<S>(p, row, at.end, at.column + quarter * 32u, raw, own, base_pointer + quarter * kStagingBytes);
         } else {
 #pragma unroll
           for (uint32_t i = 0; i < Z::kPiece; ++i) {

@@ -70,21 +70,29 @@ __device__ __forceinline__ uint32_t packed(bf16 a, bf16 b) { return (uint32_t)__
 // in sixteen bits that is nothing, and with the exact quotient the pairs of a tile took longer than its products (9.0 against 5.2 us).
 __device__ __forceinline__ float silu_short(float z) { return __fdividef(z, 1.0f + __expf(-z)); }
 
-// Sums of COUNT rows from `row` on, of the output column that is this lane's, on their way out; the whole warp takes part.  Sixteen-bit
+// Sums of COUNT rows from `row` on, of the output column that is this lane's, and its bias: fp32.
+template <int COUNT>
+__device__ __forceinline__ void store_floats(const Problem& p, uint32_t row, uint32_t end, uint32_t column, const uint32_t (&raw)[COUNT], float bias) {
+  if (column >= p.n) return;
+  float* out = reinterpret_cast<float*>(p.out) + (size_t)row * p.n + column;
+  if (row + COUNT <= end) {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i, out += p.n) *out = __uint_as_float(raw[i]) + bias;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i, out += p.n)
+    if (row + i < end) *out = __uint_as_float(raw[i]) + bias;
+}
+
+// The same in any type, on their way out; the whole warp takes part.  Sixteen-bit
 // results go two columns at a time: neighbouring lanes exchange the sums of every other row.
 template <Store S, int COUNT>
 __device__ __forceinline__ void store_rows(const Problem& p, uint32_t row, uint32_t end, uint32_t column, const uint32_t (&raw)[COUNT]) {
   typedef typename Element<S>::Type T;
   const bool odd = threadIdx.x & 1u;
   if constexpr (S == kStoreFloat) {
-    if (column >= p.n) return;
-    const float bias = p.bias ? reinterpret_cast<const float*>(p.bias)[column] : 0.0f;
-    float* out = reinterpret_cast<float*>(p.out) + (size_t)row * p.n + column;
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i, out += p.n) {
-      if (row + i >= end) break;  // the same for the whole warp
-      *out = __uint_as_float(raw[i]) + bias;
-    }
+    store_floats(p, row, end, column, raw, p.bias && column < p.n ? reinterpret_cast<const float*>(p.bias)[column] : 0.0f);
   } else {
     const uint32_t even_column = column & ~1u;
     constexpr bool kPair = S == kStorePairHalf || S == kStorePairBf16;
@@ -122,41 +130,50 @@ constexpr uint32_t kStagingRow = 80, kStagingBytes = 32 * kStagingRow;  // a war
 
 template <Store S> constexpr bool kPaired = S == kStorePairHalf || S == kStorePairBf16;
 
-// Results of sixteen bits of 16 or 32 rows from `row` on and the warp's 32 columns to shared memory, STRIDE bytes a row.
+// What a lane brings to a piece of up to 32 rows from `row` on and the warp's 32 columns: of pairs the score of its row, otherwise the bias of
+// its column, whatever the row.  Asked for ahead of the sums.
+template <Store S>
+__device__ __forceinline__ float piece_operand(const Problem& p, uint32_t row, uint32_t end, uint32_t column0) {
+  const uint32_t lane = threadIdx.x & 31u;
+  if constexpr (kPaired<S>) return row + lane < end ? p.row_scale[row + lane] : 0.0f;
+  return p.bias && column0 + lane < p.n ? as_float(reinterpret_cast<const typename Element<S>::Type*>(p.bias)[column0 + lane]) : 0.0f;
+}
+
+// Results of sixteen bits of such a piece's `rows` rows, rounded up to eights, to shared memory, STRIDE bytes a row.  A test per row kept the
+// rows' chains of operations apart: 2 us a piece of pairs, where eight rows at a time take less than a tile's products.
 template <Store S, uint32_t STRIDE, uint32_t COUNT>
-__device__ __forceinline__ void stage_piece(const Problem& p, uint32_t row, uint32_t end, uint32_t column0, const uint32_t (&raw)[COUNT], unsigned char* staging) {
+__device__ __forceinline__ void stage_piece(uint32_t rows, const uint32_t (&raw)[COUNT], float own, unsigned char* staging) {
   typedef typename Element<S>::Type T;
   const uint32_t lane = threadIdx.x & 31u;
   if constexpr (kPaired<S>) {
     const bool odd = lane & 1u;
-    const float scales = row + lane < end ? p.row_scale[row + lane] : 0.0f;
 #pragma unroll
     for (uint32_t i = 0; i < COUNT; i += 2) {
-      if (row + i >= end) break;  // the same for the whole warp
+      if (i % 8u == 0 && i >= rows) break;  // the same for the whole warp
       const uint32_t away = __shfl_xor_sync(0xffffffffu, odd ? raw[i] : raw[i + 1], 1), at = i + (odd ? 1u : 0u);
-      const float scale = __shfl_sync(0xffffffffu, scales, at);
+      const float scale = __shfl_sync(0xffffffffu, own, at);
       const float gate = __uint_as_float(odd ? away : raw[i]) * scale, up = __uint_as_float(odd ? raw[i + 1] : away) * scale;
       *reinterpret_cast<T*>(staging + at * STRIDE + lane / 2u * 2u) = from_float<T>(silu_short(gate) * up);
     }
   } else {
-    const float bias = p.bias && column0 + lane < p.n ? as_float(reinterpret_cast<const T*>(p.bias)[column0 + lane]) : 0.0f;
 #pragma unroll
     for (uint32_t i = 0; i < COUNT; ++i) {
-      if (row + i >= end) break;
-      *reinterpret_cast<T*>(staging + i * STRIDE + lane * 2u) = from_float<T>(__uint_as_float(raw[i]) + bias);
+      if (i % 8u == 0 && i >= rows) break;  // the same for the whole warp
+      *reinterpret_cast<T*>(staging + i * STRIDE + lane * 2u) = from_float<T>(__uint_as_float(raw[i]) + own);
     }
   }
 }
 
 // The same on their way out: lanes share the 64 bytes (of pairs 32) of a row.
 template <Store S, uint32_t COUNT>
-__device__ __forceinline__ void store_piece(const Problem& p, uint32_t row, uint32_t end, uint32_t column0, const uint32_t (&raw)[COUNT], unsigned char* staging) {
+__device__ __forceinline__ void store_piece(const Problem& p, uint32_t row, uint32_t end, uint32_t column0, const uint32_t (&raw)[COUNT], float own,
+                                            unsigned char* staging) {
   typedef typename Element<S>::Type T;
   const uint32_t lane = threadIdx.x & 31u;
   if constexpr (S == kStoreFloat) {
-    store_rows<S>(p, row, end, column0 + lane, raw);
+    store_floats(p, row, end, column0 + lane, raw, own);
   } else {
-    stage_piece<S, kStagingRow>(p, row, end, column0, raw, staging);
+    stage_piece<S, kStagingRow>(end - row, raw, own, staging);
     __syncwarp();
     constexpr uint32_t kVectors = kPaired<S> ? 2 : 4;  // of a row
     const uint32_t columns = kPaired<S> ? p.n / 2u : p.n, first = (kPaired<S> ? column0 / 2u : column0) + lane % kVectors * 8u;

@@ -294,6 +294,8 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     for (uint32_t tile = pair; tile < tiles && ok; tile += pairs, ++turn) {
       const uint32_t which = turn % kSums;
       const Place at = place(tile);
+      const uint32_t column = at.column + rank * kColumns + quarter * 32u;
+      float own = piece_operand<S>(p, at.row + side * 32u, at.end, column);
       ok = !*abort_flag && warp_wait(sums_full + which * 8, (turn / kSums) & 1u);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
@@ -301,25 +303,27 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t address = tmem_base + which * kMostRows + ((quarter * 32u) << 16), column = at.column + rank * kColumns + quarter * 32u;
+      const uint32_t address = tmem_base + which * kMostRows + ((quarter * 32u) << 16);
 #pragma unroll 1
       for (uint32_t piece = side; piece < kLoneRows / 32u; piece += kEpilogueWarps / 4u) {
         const uint32_t row = at.row + piece * 32u;
         if (row >= at.end) break;
         uint32_t raw[32];
         tmem_load_32(address + piece * 32u, raw);
+        const float mine = own;
+        if (kPaired<S>) own = piece_operand<S>(p, row + kEpilogueWarps / 4u * 32u, at.end, column);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         constexpr uint32_t kWidth = kPaired<S> ? 16 : 32;  // columns of results
         const uint32_t out_column = kPaired<S> ? column / 2u : column, columns = kPaired<S> ? p.n / 2u : p.n;
         if (lane == 0) await_box();
         __syncwarp();
         if (S != kStoreFloat && work.boxes && row + 32u <= at.end && out_column + kWidth <= columns) {
-          if constexpr (S != kStoreFloat) stage_piece<S, kWidth * 2>(p, row, at.end, column, raw, staging);
+          if constexpr (S != kStoreFloat) stage_piece<S, kWidth * 2>(32u, raw, mine, staging);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) store_box(&map_out, (int32_t)out_column, (int32_t)row, smem_u32(staging));
         } else {
-          store_piece<S>(p, row, at.end, column, raw, staging);
+          store_piece<S>(p, row, at.end, column, raw, mine, staging);
         }
         __syncwarp();  // tcgen05.ld needs the whole warp
       }
