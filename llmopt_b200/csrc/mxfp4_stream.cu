@@ -49,8 +49,6 @@ uint32_t shared_bytes(const Work& work) {
   return 1024u + work.stages * Z::kStageBytes + Z::kBehind + (work.splits > 1u ? (work.splits * work.share + 1u) * kColumns * 4u : 0u);
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_store(uint32_t local, uint32_t rank, uint32_t value) {
   uint32_t remote;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));

@@ -33,6 +33,9 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, barrier_wait(bar, parity)); }
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // kind::mxf4, e2m1 A and B (format 1), e8m0 scales, both K-major; `pair` picks the half of a scale word.
 __device__ __forceinline__ uint32_t mxf4_instruction(uint32_t m, uint32_t n, uint32_t pair) {
   return (pair << 5) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 4) << 24) | (pair << 30);

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_out,
              const __grid_constant__ Problem p, const Work work, uint32_t* error_word) {
   extern __shared__ unsigned char shared_raw[];
-  grid_chain_prologue();
+  grid_launch_dependents();
   const uint32_t base = (smem_u32(shared_raw) + 1023u) & ~1023u;
   unsigned char* base_pointer = shared_raw + (base - smem_u32(shared_raw));
   const uint32_t full = base, scales_full = full + kMostStages * 8, empty = scales_full + kMostStages * 8;
@@ -105,13 +105,6 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
   volatile uint32_t* holder = reinterpret_cast<volatile uint32_t*>(base_pointer + kHolder);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(base_pointer + kAbort);
   const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u, rank = blockIdx.x & 1u, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const uint32_t row_tiles = p.plan.tiles ? min(p.plan.tiles[0], work.row_tiles) : work.row_tiles;
-  const uint32_t tiles = row_tiles * work.column_tiles, k_stages = (p.k + kDepth - 1u) / kDepth;
-  auto place = [&](uint32_t tile) { return place_of(p, tile % row_tiles, work.rows, tile / row_tiles * 2u * kColumns); };
-  const uint32_t half_bytes = work.rows / 2u * kRowBytes;
-  // rows that a product takes, half of them from either CTA
-  auto width = [&](const Place& at) { return max((at.end - at.row + 31u) / 32u * 32u, 32u); };
-
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < work.stages; ++s) {
       barrier_init(full + s * 8, 1);  // of the first CTA, for both: its expect_tx arrival; completes by byte count
@@ -126,15 +119,28 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     *abort_flag = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + kHolder), "r"(kTmemColumns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  __syncwarp();
+  cluster_arrive();
+  grid_dependency_wait();  // ahead of tensor memory, which CTAs of the kernel before may still have to ask for
+  // Copies and exponents start without tensor memory, which warp 1 and the warps that store wait for.
+  uint32_t tmem_base = 0;
+  if (warp == 1u || warp >= 2u + kScaleWarps) {
+    if (warp == 1u) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + kHolder), "r"(kTmemColumns) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"((1 + kEpilogueWarps) * 32) : "memory");
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    tmem_base = uniform(*holder);
   }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  cluster_sync();  // either CTA's barriers are there for the other
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem_base = uniform(*holder);
+  cluster_wait();  // either CTA's barriers are there for the other
+  const uint32_t row_tiles = p.plan.tiles ? min(p.plan.tiles[0], work.row_tiles) : work.row_tiles;
+  const uint32_t tiles = row_tiles * work.column_tiles, k_stages = (p.k + kDepth - 1u) / kDepth;
+  auto place = [&](uint32_t tile) { return place_of(p, tile % row_tiles, work.rows, tile / row_tiles * 2u * kColumns); };
+  const uint32_t half_bytes = work.rows / 2u * kRowBytes;
+  // rows that a product takes, half of them from either CTA
+  auto width = [&](const Place& at) { return max((at.end - at.row + 31u) / 32u * 32u, 32u); };
   auto give_up = [&]() {
     *abort_flag = 1u;
     if (error_word) atomicExch(error_word, 1u);
