@@ -319,7 +319,7 @@ int run(const KernelArgs& args, const Problem& p, uint32_t row_tiles) {
   work.share = (rows + work.splits - 1u) / work.splits;
   while (shared_bytes<NT>(work) > kMostShared) --work.stages;
   auto kernel = stream_kernel<NT, S>;
-  LLMOPT_REQUIRE(allow_shared(kernel, kMostShared), "shared memory request was refused");
+  LLMOPT_REQUIRE((allow_shared<stream_kernel<NT, S>, kMostShared>()), "shared memory request was refused");
   CUtensorMap map_w, map_x;
   LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.box_rows), "tensor map was refused");
   const dim3 grid((uint32_t)tiles * work.splits);

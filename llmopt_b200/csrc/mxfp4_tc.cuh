@@ -7,6 +7,8 @@
 #pragma once
 #include <cuda.h>
 
+#include <atomic>
+
 #include "mxfp4.cuh"
 #include "w4a16_tc_device.cuh"
 
@@ -233,21 +235,35 @@ inline bool make_map(CUtensorMap* map, CUtensorMapDataType type, uint32_t size, 
   if (encode == nullptr) return false;
   const cuuint64_t dims[2] = {inner, rows}, strides[1] = {inner * size};
   const cuuint32_t box[2] = {box_inner, box_rows}, element_strides[2] = {1, 1};
-  return encode(map, type, 2, const_cast<void*>(base), dims, strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  auto made = [&] {
+    return encode(map, type, 2, const_cast<void*>(base), dims, strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (made()) return true;
+  // a thread that has called nothing yet has no context, which this call does not give it
+  int device = 0;
+  return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && made();
 }
 // Codes [rows, k / 2] read in boxes of 128 bytes x `box_rows` with the 128-byte swizzle; absent bytes read zero.
 inline bool make_map(CUtensorMap* map, const void* codes, uint64_t k, uint64_t rows, uint32_t box_rows) {
   return make_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1u, codes, k / 2, rows, kRowBytes, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Lets a kernel have as much shared memory as any launch of it asks for: the limit is one per kernel, whoever launches it.  Ahead of make_map, whose call
-// does not give a thread its context as this one does.
-template <typename... Params>
-bool allow_shared(void (*kernel)(Params...), uint32_t bytes) {
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess) return true;
-  cudaGetLastError();
-  return false;
+// Lets a kernel have as much shared memory as any launch of it asks for: the limit is one per kernel and device, whoever launches it, and the
+// call that sets it takes 0.3 us, so it is made once.
+template <auto KERNEL, uint32_t BYTES>
+bool allow_shared() {
+  static std::atomic<uint64_t> allowed{0};  // a bit per device
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  const uint64_t bit = device < 64 ? 1ull << device : 0ull;
+  if (allowed.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BYTES) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  allowed.fetch_or(bit, std::memory_order_relaxed);
+  return true;
 }
 
 inline uint32_t most_plan_tiles(uint32_t slots, uint32_t experts) { return slots / kExpertTile + (slots < experts ? slots : experts); }

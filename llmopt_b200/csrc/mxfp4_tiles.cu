@@ -373,7 +373,7 @@ int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
   work.ring = kFront + (tiles > pairs ? kStaging : 0u);
   work.stages = (kMostShared - 1024u - work.ring) / work.stage_bytes;
   if (work.stages > kMostStages) work.stages = kMostStages;
-  LLMOPT_REQUIRE(allow_shared(tiles_kernel<S>, kMostShared), "shared memory request was refused");
+  LLMOPT_REQUIRE((allow_shared<tiles_kernel<S>, kMostShared>()), "shared memory request was refused");
   CUtensorMap map_w, map_x;
   LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.rows / 2u), "tensor map was refused");
   CUtensorMap map_out = map_x;  // not read without boxes
