@@ -9,13 +9,14 @@
 // (output columns), while the next tile's are formed in other columns of tensor memory; results of 16 bits change places in shared
 // memory and leave as boxes of 32 rows by TMA, ragged ones by vector stores.
 //
-// What bounds it: a stage costs the tensor cores 4 cycles per row of x, about 50 per copy of exponents (they share the pipe: 12 of them)
-// and a handover of the ring, together close to 500 + 4 rows.  Stages of 512 rather than 256 elements halve the handovers: 4096 x
-// 4096 x 14336 108 -> 99 us, 2048 x 4096 x 4096 24.9 -> 21.3, 512 x 14336 x 4096 25.7 -> 20.9.  The large product then runs at 4.86
-// PFLOP/s, and k 8192 at 5.45; repeated for a second it draws the part's 1000 W and takes 111 us at 1.6 to 1.7 GHz.  Rows sorted by expert
-// have tiles of 128, which spend half a stage outside the products: 4096 of 16 experts through 4096 x 7168 88 us, 2.7 PFLOP/s and 2.9
-// TB/s.  Joined into tiles of up to 224 they took 87, but rows of 64 experts 116 where these take 106: taller boxes leave three stages for
-// four.
+// What bounds it: a stage costs the tensor cores 4 cycles per row of x and 200 to 500 for copies of exponents (12 of them, in the same
+// pipe) and the handover of the ring.  Stages of 512 rather than 256 elements halve the handovers: 4096 x 4096 x 14336 108 -> 99 us, 2048 x
+// 4096 x 4096 24.9 -> 21.3, 512 x 14336 x 4096 25.7 -> 20.9.  The large product takes 95 to 101 us, up to 5 PFLOP/s (k 8192: 5.4), and 80 where
+// all codes are zero: what is left between the two is power, 1000 W, and repeated for a second it takes 110 at 1.6 to 1.7 GHz.  Rows
+// sorted by expert have tiles of 128, which spend up to half a stage outside the products: 4096 of 16 experts through 4096 x 7168 80 to 83 us,
+// 2.9 PFLOP/s and 2.9 TB/s.  Joined into tiles of up to 224 they took as long, but rows of 64 experts 116 where these took 106: taller boxes
+// leave three stages for four.  Small products are bound by their ends: 128 rows through 4096 x 14336 11.9 us, 777 x 2048 x 7168 11.3; copies and
+// exponents start without waiting for tensor memory (0.5 us).
 //
 // Every wait on an mbarrier is bounded; a wait that runs out raises the context's device error word, and the CTA lets its copies and
 // products end, frees its tensor memory and returns.
