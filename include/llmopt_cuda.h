@@ -277,8 +277,8 @@ int llmopt_cuda_w4a16_linear(llmopt_cuda_context* context, const void* input, co
  *   codes  u8 [rows, k / 2], the element of even k in the low nibble, 16-byte aligned, and
  *   scales u32 [ceil(k / 128), rows]: byte j of word (g, r) is the exponent (plus 127; 255: no number) of block 4 g + j of row r;
  * k is a multiple of 32.  The kernels of the same names (llmopt_mxfp4_quantize_f16 and so on) do the same for buffers in
- * batches and plans; these run one of them on `stream` (a cudaStream_t; NULL = the context's) of the context's device without waiting,
- * keep nothing between calls and use no memory but the operands, so calls on different streams may overlap and a stream capture
+ * batches and plans; these run one of them on `stream` (a cudaStream_t; NULL = the default stream) of the context's device without
+ * waiting, keep nothing between calls and use no memory but the operands, so calls on different streams may overlap and a stream capture
  * may hold them.  `type`: what the operand without codes is held in. */
 #define LLMOPT_CUDA_F16 0
 #define LLMOPT_CUDA_BF16 1

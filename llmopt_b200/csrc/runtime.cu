@@ -1627,7 +1627,7 @@ struct PointerLaunch {
 
   PointerLaunch(Context* context, void* stream) {
     args.ctx = context;
-    args.stream = stream ? (cudaStream_t)stream : context->stream;
+    args.stream = (cudaStream_t)stream;
     args.params = (const uint8_t*)params;
     args.error = &message;
   }

@@ -412,8 +412,8 @@ class Runtime:
         _check(load_library().llmopt_cuda_w4a16_linear(
             self._context, x_ptr, packed_ptr, scale_ptr, bias_ptr or None, out_ptr, m, n, k, stream or None))
 
-    # MXFP4 operators on raw device pointers and a caller's stream (0: the context's), without waiting; formats and rounding:
-    # include/llmopt_cuda.h. ``element`` is "f16", "bf16" or "f32": what the operand outside of the 4-bit format is held in.
+    # MXFP4 operators on raw device pointers and a caller's stream (0: the default stream, as torch names its own), without waiting;
+    # formats and rounding: include/llmopt_cuda.h. ``element`` is "f16", "bf16" or "f32": what the operand outside of the 4-bit format is held in.
     _ELEMENTS = {"f16": 0, "bf16": 1, "f32": 2}
 
     def mxfp4_quantize_pointers(self, element: str, x_ptr: int, row_of_slot_ptr: Optional[int], codes_ptr: int, scales_ptr: int,

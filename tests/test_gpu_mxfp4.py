@@ -270,6 +270,61 @@ def test_products_at_the_ends_of_the_exponents(runtime, m):
         assert (np.abs(got.astype(np.float64) - exact)[~held] < 2.0 ** -149).all(), (sx, sw)
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 256, 4096), (5, 264, 96), (33, 128, 1024), (64, 1000, 512), (70, 256, 320), (300, 272, 640)])
+def test_results_and_biases_at_any_multiple_of_their_element(runtime, m, n, k):
+    from llmopt_b200 import dispatch
+
+    rng = np.random.default_rng(m + n)
+    x, w = random_operand(rng, m, k), random_operand(rng, n, k)
+    x = x[0], (x[1] - 6).astype(np.uint8)
+    xv, wv = mx.values(*x), mx.values(*w)
+    want = xv @ wv.T
+    bias = rng.standard_normal(n) * np.abs(want).max()
+    xt, wt = upload(runtime, x, 255), upload(runtime, w, 255)
+    for dtype in ("float16", "bfloat16", "float32"):
+        for steps in (1, 2, 7):
+            whole, held = blank(runtime, (m * n + steps,), dtype, 256), to_bits(bias, dtype)
+            y = dispatch.Tensor(whole.buffer.view(steps * size_of(dtype), m * n * size_of(dtype) + 256), (m, n), dtype)
+            dispatch.dispatch_mxfp4_linear(context(runtime), input=xt[0], input_scales=xt[1], weight=wt[0], weight_scales=wt[1], output=y,
+                                           bias=device(runtime, held, dtype, steps * size_of(dtype)))
+            exact = want + from_bits(held, dtype)
+            check(from_bits(read(y, 256), dtype), exact, allowed(xv, wv, exact, dtype) + 2.0 ** -23 * np.abs(exact))
+            assert (np.frombuffer(whole.buffer.contents(), np.uint8)[:steps * size_of(dtype)] == CANARY).all()
+
+
+def test_offsets_beyond_32_bits(runtime):
+    """More than 2^32 values: the first and last rows of conversions both ways, and of a product."""
+    import torch
+
+    torch.cuda.init()
+    rows, k = 2 ** 22 + 5, 1024
+    generator = torch.Generator("cuda").manual_seed(1)
+    codes = torch.randint(0, 256, (rows, k // 2), dtype=torch.uint8, device="cuda", generator=generator)
+    scales = torch.randint(120, 130, (k // 128, rows, 4), dtype=torch.uint8, device="cuda", generator=generator)
+    values = torch.empty(rows, k, dtype=torch.float16, device="cuda")
+    again, words = torch.empty_like(codes), torch.empty(k // 128, rows, dtype=torch.int32, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    runtime.mxfp4_dequantize_pointers("f16", codes.data_ptr(), scales.data_ptr(), values.data_ptr(), rows, k, stream)
+    runtime.mxfp4_quantize_pointers("f16", values.data_ptr(), None, again.data_ptr(), words.data_ptr(), rows, rows, k, k, stream)
+    for part in (slice(0, 40), slice(rows - 40, rows)):
+        want = mx.values(mx.unpack(codes[part].cpu().numpy()), mx.exponents(np.ascontiguousarray(scales[:, part].cpu().numpy()).view(np.uint32)[..., 0], k))
+        assert np.array_equal(values[part].cpu().double().numpy(), want)
+        nibbles, exponents = mx.quantize(want)
+        assert np.array_equal(again[part].cpu().numpy(), mx.pack(nibbles))
+        assert np.array_equal(np.ascontiguousarray(words[:, part].cpu().numpy()).view(np.uint32), mx.words(exponents))
+    del values, again
+    m, n = 4099, 2 ** 20 + 8
+    x, w = codes.view(-1)[:m * 16], codes.view(-1)[-n * 16:]  # k of 32
+    xs, ws = (torch.full((1, rows, 4), 125, dtype=torch.uint8, device="cuda")[:, :count].contiguous() for count in (m, n))
+    y = torch.empty(m, n, dtype=torch.float16, device="cuda")
+    runtime.mxfp4_linear_pointers("f16", x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), None, y.data_ptr(), m, n, 32, stream)
+    value = lambda held, count: mx.values(mx.unpack(held.cpu().numpy().reshape(count, 16)), np.full((count, 1), 125, np.uint8))
+    wv = value(w, n)
+    for row in (0, m // 2, m - 1):  # whole sixty-fourths of at most 72, which 16 bits hold to 11 bits of fraction
+        want = (value(x[row * 16:row * 16 + 16], 1) @ wv.T)[0]
+        assert np.array_equal(y[row].cpu().numpy(), want.astype(np.float16))
+
+
 @pytest.mark.parametrize("m,n,k", [(3, 200, 416), (40, 130, 4096), (300, 260, 1024)])
 def test_blocks_of_nan_reach_their_row_or_column_alone(runtime, m, n, k):
     from llmopt_b200 import dispatch
@@ -647,6 +702,36 @@ def test_pointers_streams_and_captured_calls(runtime):
         torch.cuda.synchronize()
         for c, x in zip(cases, inputs):
             checked(c, x)
+
+
+def test_calls_on_the_default_stream_come_after_its_work(runtime):
+    """A stream of 0 is torch's default one: what that still has to write is read, and what it does next reads the results."""
+    import torch
+
+    torch.cuda.init()
+    rng = np.random.default_rng(32)
+    for m in (2, 80):
+        n, k = 256, 512
+        w = random_operand(rng, n, k)
+        held = torch.from_numpy(mx.pack(w[0])).cuda(), torch.from_numpy(mx.words(w[1]).view(np.int32)).cuda()
+        x, codes = torch.zeros(m, k, device="cuda"), torch.zeros(m, k // 2, dtype=torch.uint8, device="cuda")
+        words, y = torch.zeros(k // 128, m, dtype=torch.int32, device="cuda"), torch.zeros(m, n, device="cuda")
+        values = torch.zeros(m, k, device="cuda")
+        source = torch.randn(m, k, device="cuda")
+        torch.cuda.synchronize()
+        stream = torch.cuda.current_stream().cuda_stream
+        torch.cuda._sleep(100_000_000)
+        x.copy_(source)
+        runtime.mxfp4_quantize_pointers("f32", x.data_ptr(), None, codes.data_ptr(), words.data_ptr(), m, m, k, k, stream)
+        runtime.mxfp4_dequantize_pointers("f32", codes.data_ptr(), words.data_ptr(), values.data_ptr(), m, k, stream)
+        runtime.mxfp4_linear_pointers("f32", codes.data_ptr(), words.data_ptr(), held[0].data_ptr(), held[1].data_ptr(), None, y.data_ptr(),
+                                      m, n, k, stream)
+        got, got_values = y.clone(), values.clone()
+        for tensor in (x, codes, words, values, y):
+            tensor.zero_()
+        xv, wv = mx.values(*mx.quantize(source.cpu().double().numpy())), mx.values(*w)
+        assert np.array_equal(got_values.cpu().double().numpy(), xv)
+        check(got.cpu().double().numpy(), xv @ wv.T, allowed(xv, wv, xv @ wv.T, "float32"))
 
 
 def test_calls_from_several_threads(runtime):
