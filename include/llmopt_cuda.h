@@ -279,7 +279,8 @@ int llmopt_cuda_w4a16_linear(llmopt_cuda_context* context, const void* input, co
  * k is a multiple of 32.  The kernels of the same names (llmopt_mxfp4_quantize_f16 and so on) do the same for buffers in
  * batches and plans; these run one of them on `stream` (a cudaStream_t; NULL = the default stream) of the context's device without
  * waiting, keep nothing between calls and use no memory but the operands, so calls on different streams may overlap and a stream capture
- * may hold them.  `type`: what the operand without codes is held in. */
+ * may hold them.  A wait inside a kernel that runs out is reported by the context's next wait.  `type`: what the operand without codes
+ * is held in. */
 #define LLMOPT_CUDA_F16 0
 #define LLMOPT_CUDA_BF16 1
 #define LLMOPT_CUDA_F32 2
