@@ -13,9 +13,8 @@
 // pipe) and the handover of the ring.  Stages of 512 rather than 256 elements halve the handovers: 4096 x 4096 x 14336 108 -> 99 us, 2048 x
 // 4096 x 4096 24.9 -> 21.3, 512 x 14336 x 4096 25.7 -> 20.9.  The large product takes 95 to 101 us, up to 5 PFLOP/s (k 8192: 5.4), and 80 where
 // all codes are zero: what is left between the two is power, 1000 W, and repeated for a second it takes 110 at 1.6 to 1.7 GHz.  Rows
-// sorted by expert have tiles of 128, which spend up to half a stage outside the products: 4096 of 16 experts through 4096 x 7168 80 to 83 us,
-// 2.9 PFLOP/s and 2.9 TB/s.  Joined into tiles of up to 224 they took as long, but rows of 64 experts 116 where these took 106: taller boxes
-// leave three stages for four.  Small products are bound by their ends: 128 rows through 4096 x 14336 11.9 us, 777 x 2048 x 7168 11.3; copies and
+// sorted by expert have tiles of 128, which spend up to half a stage outside the products; many are joined to tiles of up to 224: 4096 of 16
+// experts through 4096 x 7168 85 -> 73 us, 3.3 PFLOP/s and 3.1 TB/s.  Small products are bound by their ends: 128 rows through 4096 x 14336 11.9 us, 777 x 2048 x 7168 11.3; copies and
 // exponents start without waiting for tensor memory (0.5 us).
 //
 // Every wait on an mbarrier is bounded; a wait that runs out raises the context's device error word, and the CTA lets its copies and
@@ -43,7 +42,9 @@ static_assert(kSums * kMostRows + kScaleColumns <= kTmemColumns && kInputAt % 10
 // no pair has a second tile that would be on its way into it.
 constexpr uint32_t kHolder = (3 * kMostStages + 2 * kSums + 1) * 8, kAbort = kHolder + 4, kFront = 1024, kMostShared = 227 * 1024;
 constexpr uint32_t kStaging = kEpilogueWarps * kStagingBytes;
-static_assert(kAbort + 4 <= kFront && kStaging % 1024 == 0, "alignment of tiles");
+// Joined tiles of a plan: their number, then first row and expert << 16 | rows of each, in front of the staging.
+constexpr uint32_t kCount = kAbort + 4, kMostJoined = 512, kList = kMostJoined * 8;
+static_assert(kCount + 4 <= kFront && kStaging % 1024 == 0 && kList % 1024 == 0, "alignment of tiles");
 static_assert(kStagingBytes >= 32 * 64, "a box of results");
 
 struct Work {
@@ -51,6 +52,7 @@ struct Work {
   uint32_t rows;                       // most of a tile; either CTA copies half of them, whatever there are
   uint32_t stages, stage_bytes, ring;  // of shared memory; where the ring begins
   uint32_t boxes;                      // results leave in boxes
+  uint32_t list;                       // bytes of the list of joined tiles; 0: the plan's
 };
 
 // The first CTA's barriers, from either.
@@ -92,6 +94,38 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, int32_t x, int
 }
 // Until this thread's boxes have been read.
 __device__ __forceinline__ void await_box() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
+// The plan's tiles of an expert lie behind one another and have up to 128 rows: 32 of the plan's at a time, runs of one expert's are divided
+// evenly into as few as have no more than `rows`.  A warp's; no more tiles come out than went in.
+__device__ __forceinline__ void join_tiles(const Problem& p, uint32_t plan_tiles, uint32_t rows, volatile uint32_t* number, uint2* list) {
+  const uint32_t lane = threadIdx.x & 31u;
+  uint32_t made = 0, count = plan_tiles;
+  for (uint32_t base = 0; base < count; base += 32u) {
+    Place at = {};
+    if (base + lane < plan_tiles) at = place_of(p, base + lane, kExpertTile, 0u);
+    count = min(p.plan.tiles[0], plan_tiles);
+    const bool present = base + lane < count;
+    const uint32_t of_before = __shfl_up_sync(0xffffffffu, at.w_row, 1), end_before = __shfl_up_sync(0xffffffffu, at.end, 1);
+    const bool begins = lane == 0 || of_before != at.w_row || end_before != at.row;
+    // runs end ahead of the next one, or of what is not there
+    const uint32_t ends = __ballot_sync(0xffffffffu, begins || !present) & (0xfffffffeu << lane);
+    const uint32_t end = __shfl_sync(0xffffffffu, at.end, ends ? __ffs(ends) - 2 : 31);
+    const uint32_t tiles = present && begins ? (end - at.row + rows - 1u) / rows : 0u;
+    uint32_t before = tiles;
+#pragma unroll
+    for (uint32_t offset = 1; offset < 32u; offset <<= 1) {
+      const uint32_t other = __shfl_up_sync(0xffffffffu, before, offset);
+      if (lane >= offset) before += other;
+    }
+    uint2* const target = list + made + before - tiles;
+    made += __shfl_sync(0xffffffffu, before, 31);
+    if (tiles > 0) {
+      const uint32_t each = ((end - at.row + tiles - 1u) / tiles + 31u) / 32u * 32u, expert = at.w_row / p.n;
+      for (uint32_t t = 0, row = at.row; t < tiles; ++t, row += each) target[t] = make_uint2(row, expert << 16 | min(each, end - row));
+    }
+  }
+  if (lane == 0) *number = made;
+}
 
 template <Store S>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -136,9 +170,24 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     tmem_base = uniform(*holder);
   }
   cluster_wait();  // either CTA's barriers are there for the other
-  const uint32_t row_tiles = p.plan.tiles ? min(p.plan.tiles[0], work.row_tiles) : work.row_tiles;
+  uint2* const list = reinterpret_cast<uint2*>(base_pointer + kFront);
+  uint32_t row_tiles = work.row_tiles;
+  if (work.list > 0) {
+    volatile uint32_t* joined = reinterpret_cast<volatile uint32_t*>(base_pointer + kCount);
+    if (warp == 2u) join_tiles(p, work.row_tiles, work.rows, joined, list);
+    __syncthreads();
+    row_tiles = *joined;
+  } else if (p.plan.tiles) {
+    row_tiles = min(p.plan.tiles[0], work.row_tiles);
+  }
   const uint32_t tiles = row_tiles * work.column_tiles, k_stages = (p.k + kDepth - 1u) / kDepth;
-  auto place = [&](uint32_t tile) { return place_of(p, tile % row_tiles, work.rows, tile / row_tiles * 2u * kColumns); };
+  // tiles of the same weights follow one another
+  auto place = [&](uint32_t tile) -> Place {
+    const uint32_t column = tile / row_tiles * 2u * kColumns;
+    if (work.list == 0) return place_of(p, tile % row_tiles, work.rows, column);
+    const uint2 at = list[tile % row_tiles];
+    return {at.x, at.x + (at.y & 0xffffu), (at.y >> 16) * p.n + column, column};
+  };
   const uint32_t half_bytes = work.rows / 2u * kRowBytes;
   // rows that a product takes, half of them from either CTA
   auto width = [&](const Place& at) { return max((at.end - at.row + 31u) / 32u * 32u, 32u); };
@@ -295,7 +344,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     if (!ok) give_up();
   } else {
     const uint32_t worker = warp - 2u - kScaleWarps, quarter = warp & 3u, side = worker >> 2;  // lanes of tensor memory; every other piece
-    unsigned char* const staging = base_pointer + kFront + worker * kStagingBytes;
+    unsigned char* const staging = base_pointer + kFront + work.list + worker * kStagingBytes;
     uint32_t turn = 0;
     bool ok = true;
     for (uint32_t tile = pair; tile < tiles && ok; tile += pairs, ++turn) {
@@ -357,7 +406,7 @@ namespace mxfp4 {
 template <Store S>
 int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
   const uint32_t pairs = (uint32_t)context_sm_count(args.ctx) / 2u, k_stages = (p.k + kDepth - 1u) / kDepth;
-  Work work = {plan_tiles, (p.n + 2u * kColumns - 1u) / (2u * kColumns), kExpertTile, 0u, 0u, 0u, 0u};
+  Work work = {plan_tiles, (p.n + 2u * kColumns - 1u) / (2u * kColumns), kExpertTile, 0u, 0u, 0u, 0u, 0u};
   if (!p.plan.tiles) {
     // the height with the shortest estimate: rounds of tiles times the cycles of one, of which a stage takes about 500 and four per row
     uint64_t least = ~0ull;
@@ -367,11 +416,17 @@ int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
       const uint64_t rounds = ((uint64_t)row_tiles * work.column_tiles + pairs - 1u) / pairs, cost = rounds * ((uint64_t)k_stages * (500u + 4u * rows) + 1000u);
       if (cost < least) least = cost, work.rows = rows, work.row_tiles = row_tiles;
     }
+  } else if (p.m >= p.plan.experts * kExpertTile && p.k >= 4u * kDepth && plan_tiles <= kMostJoined) {
+    // The plan's tiles joined where experts have as many rows as one on average, and products enough to make up for taller boxes and one stage
+    // less.  us, the plan's and joined, through 4096 x 7168: 16384 rows of 16 experts 276, 228, 8192 of 8 137, 111, 4096 of 16 85, 73, 1024 of 8
+    // 36.0, 32.3; 16384 of 64 through 2048 x 2816 75.7, 70.3.  Fewer rows: 1024 of 16 45.7, 45.0 (through 3584 x 4096 21.3, 23.1), 4096 of 64 through
+    // 2048 x 2048 28.4, 29.9; smaller k: 16384 of 64 through 1408 x 2048 52.5, 54.4, 1200 of 8 10.4, 12.4.
+    work.rows = kMostRows, work.list = kList;
   }
   const uint64_t tiles = (uint64_t)work.row_tiles * work.column_tiles;
   LLMOPT_REQUIRE(tiles < (1u << 28), "too many tiles");
   work.stage_bytes = kInputAt + kBoxes * (work.rows / 2u * kRowBytes);
-  work.ring = kFront + (tiles > pairs ? kStaging : 0u);
+  work.ring = kFront + work.list + (tiles > pairs ? kStaging : 0u);
   work.stages = (kMostShared - 1024u - work.ring) / work.stage_bytes;
   if (work.stages > kMostStages) work.stages = kMostStages;
   LLMOPT_REQUIRE((allow_shared<tiles_kernel<S>, kMostShared>()), "shared memory request was refused");

@@ -364,7 +364,8 @@ def expert_case(rng, counts, n, k):
 EXPERTS = [([1], 2, 32), ([0, 0, 1], 64, 160), ([1, 1], 7168, 1024), ([3, 0, 1, 0, 0, 2, 1, 1], 258, 576), ([0, 5, 11, 0], 130, 2048),
            ([128, 127, 129, 0, 1], 96, 416), ([300], 200, 256), ([0, 700, 3, 0, 65], 320, 1792), ([2] * 40, 32, 96), ([17, 33, 64, 40], 500, 736),
            ([1, 3] * 12, 5400, 96), ([40, 0, 1] + [1] * 19, 6000, 544),
-           ([225, 224, 449, 1, 128], 322, 352), ([5000, 40, 0, 3000], 64, 64), ([1, 0, 400], 4736, 1056)]
+           ([225, 224, 449, 1, 128], 322, 352), ([5000, 40, 0, 3000], 64, 64), ([1, 0, 400], 4736, 1056),
+           ([225, 224, 449, 1, 128], 322, 2080), ([5000, 40, 0, 3000], 64, 2048), ([1, 0, 400], 4736, 2176), ([160] * 40, 34, 2048)]
 
 
 @pytest.mark.parametrize("case", range(len(EXPERTS)))
@@ -429,12 +430,13 @@ def test_expert_rows_without_a_tile_stay_as_they_were(runtime):
     assert np.allclose(got[6:], xv[6:] @ wv[n:].T, rtol=1e-5, atol=1e-3)
 
 
-def test_many_expert_rows_follow_the_plan(runtime):
+@pytest.mark.parametrize("k", [256, 2048])
+def test_many_expert_rows_follow_the_plan(runtime, k):
     """Rows between the tiles stay as they were, and what points outside is cut."""
     from llmopt_b200 import dispatch
 
     rng = np.random.default_rng(13)
-    n, k, slots = 96, 256, 600
+    n, slots = 96, 600
     x, w = random_operand(rng, slots, k), random_operand(rng, 2 * n, k)
     xt, wt = upload(runtime, x), upload(runtime, w)
     plan = np.zeros((1 + slots // 128 + 2, 4), np.uint32)
