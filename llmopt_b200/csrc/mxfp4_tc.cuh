@@ -169,7 +169,21 @@ __device__ __forceinline__ void stage_piece(uint32_t rows, const uint32_t (&raw)
   }
 }
 
-// The same on their way out: lanes share the 64 bytes (of pairs 32) of a row.
+// Staged rows to `out`, whose rows are `stride` elements apart: lanes share the 64 bytes (of pairs 32) of a row, a V of them each.  With eight
+// values per lane whatever the alignment, stored one by one, 3209 x 256 x 7126 took 114 us, with a V that fits 31 (7128 columns, in boxes: 16).
+template <Store S, typename V, uint32_t COUNT, typename T>
+__device__ __forceinline__ void unstage_piece(T* out, uint32_t stride, uint32_t rows, uint32_t width, const unsigned char* staging) {
+  constexpr uint32_t kValues = sizeof(V) / 2, kLanes = (kPaired<S> ? 16 : 32) / kValues;  // of a V; of a row
+  const uint32_t lane = threadIdx.x & 31u, first = lane % kLanes * kValues;
+#pragma unroll
+  for (uint32_t i = 0; i < COUNT * kLanes / 32; ++i) {
+    const uint32_t at = i * (32u / kLanes) + lane / kLanes;
+    if (at < rows && first < width)
+      *reinterpret_cast<V*>(out + (size_t)at * stride + first) = *reinterpret_cast<const V*>(staging + at * kStagingRow + first * 2u);
+  }
+}
+
+// A piece on its way out.
 template <Store S, uint32_t COUNT>
 __device__ __forceinline__ void store_piece(const Problem& p, uint32_t row, uint32_t end, uint32_t column0, const uint32_t (&raw)[COUNT], float own,
                                             unsigned char* staging) {
@@ -180,24 +194,12 @@ __device__ __forceinline__ void store_piece(const Problem& p, uint32_t row, uint
   } else {
     stage_piece<S, kStagingRow>(end - row, raw, own, staging);
     __syncwarp();
-    constexpr uint32_t kVectors = kPaired<S> ? 2 : 4;  // of a row
-    const uint32_t columns = kPaired<S> ? p.n / 2u : p.n, first = (kPaired<S> ? column0 / 2u : column0) + lane % kVectors * 8u;
-    const bool vectors = columns % 8u == 0 && ((uintptr_t)p.out & 15u) == 0;
-#pragma unroll
-    for (uint32_t i = 0; i < COUNT * kVectors / 32; ++i) {
-      const uint32_t at = i * (32u / kVectors) + lane / kVectors;
-      if (row + at >= end || first >= columns) continue;
-      const uint4 eight = *reinterpret_cast<const uint4*>(staging + at * kStagingRow + lane % kVectors * 16u);
-      T* const out = reinterpret_cast<T*>(p.out) + (size_t)(row + at) * columns + first;
-      if (vectors) {
-        *reinterpret_cast<uint4*>(out) = eight;
-      } else {
-        const T* const values = reinterpret_cast<const T*>(&eight);
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j)
-          if (first + j < columns) out[j] = values[j];
-      }
-    }
+    const uint32_t columns = kPaired<S> ? p.n / 2u : p.n, column = kPaired<S> ? column0 / 2u : column0;
+    T* const out = reinterpret_cast<T*>(p.out) + (size_t)row * columns + column;
+    const uint32_t rows = min(end - row, COUNT), width = column < columns ? columns - column : 0u;
+    if (columns % 8u == 0 && ((uintptr_t)p.out & 15u) == 0) unstage_piece<S, uint4, COUNT>(out, columns, rows, width, staging);
+    else if (columns % 2u == 0 && ((uintptr_t)p.out & 3u) == 0) unstage_piece<S, uint32_t, COUNT>(out, columns, rows, width, staging);
+    else unstage_piece<S, uint16_t, COUNT>(out, columns, rows, width, staging);
     __syncwarp();  // read before the next piece
   }
 }
