@@ -5,8 +5,8 @@
 // 44 KB.  In each CTA warp 0 brings the codes of 512 elements of k of its halves by TMA (128-byte swizzle); warps 2 to 5 bring
 // exponents, a warp per word of a stage, those of the CTA's 128 weight rows and of all rows of x, requested three stages ahead and laid
 // down in the order that tcgen05.cp spreads over tensor memory.  One lane of warp 1 of the first CTA issues copies and products
-// for both, and its barriers count both CTAs' copies and exponents.  Eight more warps read a tile's sums out, each a quarter of the lanes
-// (output columns), while the next tile's are formed in other columns of tensor memory; results of 16 bits change places in shared
+// for both, and its barriers count both CTAs' copies and exponents (the second one's when its warp 1 says so).  Eight more warps read a
+// tile's sums out, each a quarter of the lanes (output columns), while the next tile's are formed in other columns of tensor memory; results of 16 bits change places in shared
 // memory and leave as boxes of 32 rows by TMA, ragged ones by vector stores.
 //
 // What bounds it: a stage costs the tensor cores 4 cycles per row of x and 200 to 500 for copies of exponents (12 of them, in the same
@@ -40,7 +40,7 @@ constexpr uint32_t kWordColumns = 4 * (1 + kInputAtoms), kScaleColumns = kStageW
 static_assert(kSums * kMostRows + kScaleColumns <= kTmemColumns && kInputAt % 1024 == 0, "tensor memory, alignment of tiles");
 // In front of the ring: barriers, tensor memory's address, abort flag, and the staging of the warps that store, which lies over the ring where
 // no pair has a second tile that would be on its way into it.
-constexpr uint32_t kHolder = (3 * kMostStages + 2 * kSums + 1) * 8, kAbort = kHolder + 4, kFront = 1024, kMostShared = 227 * 1024;
+constexpr uint32_t kHolder = (5 * kMostStages + 2 * kSums + 1) * 8, kAbort = kHolder + 4, kFront = 1024, kMostShared = 227 * 1024;
 constexpr uint32_t kStaging = kEpilogueWarps * kStagingBytes;
 // Joined tiles of a plan: their number, then first row and expert << 16 | rows of each, in front of the staging.
 constexpr uint32_t kCount = kAbort + 4, kMostJoined = 512, kList = kMostJoined * 8;
@@ -61,7 +61,30 @@ __device__ __forceinline__ uint32_t first_address(uint32_t local) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(0u));
   return remote;
 }
-__device__ __forceinline__ void first_arrive(uint32_t first) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(first) : "memory"); }
+// The two CTAs hand each other shared memory (exponents laid down, stages read) and tensor memory (sums read out) by barriers whose arrivals and
+// waits have to be of the cluster's scope: one that names none is the CTA's, and orders nothing between threads of two CTAs.  They are relaxed,
+// with fences restricted to shared memory where that changes hands and tcgen05.fence for tensor memory: release and acquire of
+// everything wait for global memory too.  The warps that bring exponents take part in none of it: even a restricted fence waits for the loads that
+// they have under way, so warp 0 tells them when a stage is theirs, and the second CTA's warp 1 tells the first what they have laid down.
+// us, cold, of 777 x 2048 x 7168, 4096 x 4096 x 14336 and 32 x 4096 x 128256 (fp32): 10.4, 93, 48.3; with fences in those warps 10.8, 98, 55; with
+// release and acquire of everything 15.4, 156, 87.
+__device__ __forceinline__ void shared_release() { asm volatile("fence.release.sync_restrict::shared::cta.cluster;" ::: "memory"); }
+__device__ __forceinline__ void first_arrive(uint32_t first) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(first) : "memory");
+}
+__device__ __forceinline__ bool pair_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done = 0;
+  for (uint32_t spin = 0; spin < kWaitLimit && !done; ++spin)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+  asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
+  return __all_sync(0xffffffffu, done != 0u);
+}
 // A tile to this CTA's shared memory whose bytes the barrier of the first one counts.
 __device__ __forceinline__ void pair_load(uint32_t destination, const CUtensorMap* map, int32_t x, int32_t y, uint32_t first) {
   asm volatile(
@@ -137,13 +160,16 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
   unsigned char* base_pointer = shared_raw + (base - smem_u32(shared_raw));
   const uint32_t full = base, scales_full = full + kMostStages * 8, empty = scales_full + kMostStages * 8;
   const uint32_t sums_full = empty + kMostStages * 8, sums_empty = sums_full + kSums * 8, drained = sums_empty + kSums * 8;
+  const uint32_t laid = drained + 8, vacant = laid + kMostStages * 8;
   volatile uint32_t* holder = reinterpret_cast<volatile uint32_t*>(base_pointer + kHolder);
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(base_pointer + kAbort);
   const uint32_t warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31u, rank = blockIdx.x & 1u, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < work.stages; ++s) {
       barrier_init(full + s * 8, 1);  // of the first CTA, for both: its expect_tx arrival; completes by byte count
-      barrier_init(scales_full + s * 8, 2 * kScaleWarps);  // the same
+      barrier_init(scales_full + s * 8, kScaleWarps + 1);  // the same: its own warps, and warp 1 of the second CTA for that one's
+      barrier_init(laid + s * 8, kScaleWarps);  // of the second CTA
+      barrier_init(vacant + s * 8, 1);          // warp 0's word to the warps that bring exponents: the stage is empty
       barrier_init(empty + s * 8, 1);  // one tcgen05.commit
     }
     for (uint32_t s = 0; s < kSums; ++s) {
@@ -204,13 +230,14 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       const uint32_t x_row = uniform(at.row + rank * (width(at) / 2u)), w_row = uniform(at.w_row) + rank * kColumns;
       for (uint32_t ks = 0; ks < k_stages; ++ks, ++issued) {
         const uint32_t stage = base + work.ring + s * work.stage_bytes, boxes = min(kBoxes, (p.k - ks * kDepth + kBoxDepth - 1u) / kBoxDepth);
-        ok = !*abort_flag && warp_wait(empty + s * 8, phase);
+        ok = !*abort_flag && pair_wait(empty + s * 8, phase);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) {
           give_up();
           break;
         }
         if (elect_one()) {
+          barrier_arrive(vacant + s * 8);
           const uint32_t first = first_address(full + s * 8);
           if (rank == 0u) barrier_expect_tx(full + s * 8, 2u * boxes * (kBoxBytes + half_bytes));
           for (uint32_t box = 0; box < boxes; ++box) {
@@ -232,7 +259,22 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       for (uint32_t i = 0; i < 1000u; ++i) __nanosleep(1000);
     __syncwarp();
   } else if (warp == 1 && rank == 1u) {
-    // the first CTA issues for both
+    // the first CTA issues for both, and hears from here that exponents lie in the second one's memory
+    uint32_t s = 0, phase = 0;
+    bool ok = true;
+    for (uint32_t tile = pair; tile < tiles && ok; tile += pairs)
+      for (uint32_t ks = 0; ks < k_stages; ++ks) {
+        ok = !*abort_flag && warp_wait(laid + s * 8, phase);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) {
+          shared_release();
+          first_arrive(first_address(scales_full + s * 8));
+        }
+        __syncwarp();
+        if (++s == work.stages) s = 0, phase ^= 1u;
+      }
+    if (!ok) give_up();
   } else if (warp == 1) {
     uint32_t s = 0, phase = 0, turn = 0;
     bool ok = true;
@@ -240,12 +282,12 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       const uint32_t rows = uniform(width(place(tile)));
       const uint32_t low = mxf4_instruction(2u * kColumns, rows, 0u), high = mxf4_instruction(2u * kColumns, rows, 1u);
       const uint32_t which = turn % kSums, sums = tmem_base + which * kMostRows, scales = tmem_base + kSums * kMostRows;
-      ok = !*abort_flag && warp_wait(sums_empty + which * 8, ((turn / kSums) & 1u) ^ 1u);
+      ok = !*abort_flag && pair_wait(sums_empty + which * 8, ((turn / kSums) & 1u) ^ 1u);
       ok = __all_sync(0xffffffffu, ok);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       for (uint32_t ks = 0; ks < k_stages && ok; ++ks) {
         const uint32_t stage = base + work.ring + s * work.stage_bytes;
-        ok = !*abort_flag && warp_wait(full + s * 8, phase) && warp_wait(scales_full + s * 8, phase);
+        ok = !*abort_flag && pair_wait(full + s * 8, phase) && pair_wait(scales_full + s * 8, phase);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -280,7 +322,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       if (elect_one())
         asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drained) : "memory");
       __syncwarp();
-      warp_wait(drained, 0u);
+      pair_wait(drained, 0u);
     }
   } else if (warp < 2u + kScaleWarps) {
     // the words of group warp - 2 of a stage, of the CTA's weight rows and of the tile's rows of x: lane, lane + 32, ...
@@ -315,13 +357,13 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     };
 #pragma unroll
     for (uint32_t a = 0; a < kAhead; ++a) fetch(held[a]);
-    uint32_t s = 0, phase = 1, ks = 0;
+    uint32_t s = 0, phase = 0, ks = 0;
     bool ok = true;
     for (uint32_t first = 0; first < all && ok; first += kAhead) {
 #pragma unroll
       for (uint32_t a = 0; a < kAhead; ++a) {
         if (first + a >= all || !ok) break;
-        ok = !*abort_flag && warp_wait(empty + s * 8, phase);
+        ok = !*abort_flag && warp_wait(vacant + s * 8, phase);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint32_t mask = ks * kStageWords + group + 1u == words ? last_mask : 0xffffffffu;
@@ -335,7 +377,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         line(kInputScalesAt + (group * kInputAtoms + 1u) * kAtom, 8u);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) first_arrive(first_address(scales_full + s * 8));
+        if (lane == 0) barrier_arrive((rank == 0u ? scales_full : laid) + s * 8);
         fetch(held[a]);
         if (++ks == k_stages) ks = 0;
         if (++s == work.stages) s = 0, phase ^= 1u;
@@ -352,7 +394,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       const Place at = place(tile);
       const uint32_t column = at.column + rank * kColumns + quarter * 32u;
       float own = piece_operand<S>(p, at.row + side * 32u, at.end, column);
-      ok = !*abort_flag && warp_wait(sums_full + which * 8, (turn / kSums) & 1u);
+      ok = !*abort_flag && pair_wait(sums_full + which * 8, (turn / kSums) & 1u);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
         give_up();
