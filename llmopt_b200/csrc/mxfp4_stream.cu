@@ -10,8 +10,8 @@
 // latency and the way out are half of it; 4096 x 4096 5.6.  Stages of 256 had the same bytes in flight and twice the handovers, 485 cycles
 // each, more than the copies of a stage take.  Asking for the weights while the previous kernel ends made both slower.
 //
-// Every wait on an mbarrier is bounded; a wait that runs out raises the context's device error word, and the CTA lets its copies land,
-// frees its tensor memory and returns.
+// Every wait on an mbarrier is bounded; a wait that runs out raises the context's device error word, and the CTA lets its copies and
+// products end, frees its tensor memory and returns.
 #include "mxfp4_tc.cuh"
 
 namespace llmopt {
@@ -84,7 +84,7 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
         barrier_init(empty + s * 8, 1);  // one tcgen05.commit
       }
       barrier_init(sums_full, 1);  // one tcgen05.commit
-      barrier_init(drained, 1);    // the same, where a CTA gives up
+      barrier_init(drained, 1);    // the same, where somebody gave up
       *abort_flag = 0u;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -150,9 +150,10 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
   }
   const uint32_t tmem_base = warp > 0 ? uniform(*holder) : 0u;
 
+  uint32_t issued = min(work.stages, stage1 - stage0);  // stages, by warp 0
   if (warp == 0) {
     bool ok = true;
-    uint32_t s = 0, phase = 0, issued = min(work.stages, stage1 - stage0);
+    uint32_t s = 0, phase = 0;
     for (uint32_t ks = stage0 + issued; ks < stage1; ++ks, ++issued) {
       ok = !*abort_flag && warp_wait(empty + s * 8, phase);
       ok = __all_sync(0xffffffffu, ok);
@@ -163,11 +164,6 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
       load(ks, s);
       if (++s == work.stages) s = 0, phase ^= 1u;
     }
-    // on the way out after a failure the copies already started must land first
-    if (!ok || *abort_flag)
-      for (uint32_t i = issued > work.stages ? issued - work.stages : 0u; i < issued; ++i)
-        barrier_wait(full + (i % work.stages) * 8, (i / work.stages) & 1u);
-    __syncwarp();
   } else if (warp == 1) {
     const uint32_t rows = p.plan.tiles ? uniform(max((at.end - at.row + 15u) / 16u * 16u, 16u)) : NT;
     const uint32_t low = mxf4_instruction(kColumns, rows, 0u), high = mxf4_instruction(kColumns, rows, 1u);
@@ -201,12 +197,7 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
       __syncwarp();
       if (++s == work.stages) s = 0, phase ^= 1u;
     }
-    if (!ok) {
-      give_up();
-      if (elect_one()) mma_commit(drained);  // the products already issued read the ring
-      __syncwarp();
-      warp_wait(drained, 0u);
-    }
+    if (!ok) give_up();
   } else {
     const uint32_t group = warp - 2u, last_mask = last_word_mask(p.k);
     bool ok = true;
@@ -275,6 +266,19 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
   if (warp < 2u && splits > 1u) cluster_wait();
 
   __syncthreads();
+  // Whoever gave up has said so by now.  What was started then must end before the CTA leaves its shared and tensor memory to others: copies, of
+  // which those that nobody waited for are among the ring's last, and products.
+  if (*abort_flag) {
+    if (warp == 0) {
+      for (uint32_t i = issued > work.stages ? issued - work.stages : 0u; i < issued; ++i)
+        barrier_wait(full + (i % work.stages) * 8, (i / work.stages) & 1u);
+    } else if (warp == 1) {
+      if (elect_one()) mma_commit(drained);
+      __syncwarp();
+      warp_wait(drained, 0u);
+    }
+    __syncwarp();
+  }
   // Before CTAs of a cluster wait for one another's sums: one that waits for columns which another grid holds must not be waited for with
   // these held.
   if (warp == 1) {

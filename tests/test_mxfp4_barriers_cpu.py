@@ -1,4 +1,4 @@
-"""Every order in which the warps of the MXFP4 products (csrc/mxfp4_tiles.cu) can reach their barriers, on a model.  A wait on an mbarrier
+"""Every order in which the warps of the MXFP4 products (csrc/mxfp4_stream.cu, mxfp4_tiles.cu) can reach their barriers, on a model.  A wait on an mbarrier
 names a phase by its parity alone, so it is right only while nobody is two phases behind; copies and products are asynchronous."""
 
 import os
@@ -75,6 +75,94 @@ class Model:
                 wrong.add("stuck")
             pending.extend(following)
         return wrong
+
+
+    def ways_out(self, leave):
+        """The same where any wait can run out: its warp ends there (place p becomes ~p).  States whose warps all have ended, some by
+        giving up, are handed to ``leave``, which says what can go wrong from there on."""
+        wrong, seen, pending = set(), set(), [self.start]
+        while pending:
+            state = pending.pop()
+            if state in seen:
+                continue
+            seen.add(state)
+            pending.extend(self.events(state))
+            places, ended = state[0], True
+            for warp, program in enumerate(self.programs):
+                place = places[warp]
+                if place == len(program) or place < 0:
+                    continue
+                ended = False
+                barrier, phase, effects = program[place]
+                ends, over = self.passes(state, barrier, phase)
+                if ends and not over:
+                    wrong.add("early")
+                elif ends:
+                    pending.append(self.effects(state, warp, effects))
+                if barrier is not None:
+                    pending.append((places[:warp] + (~place,) + places[warp + 1:], *state[1:]))
+            if ended and min(places) < 0:
+                wrong |= leave(state)
+        return wrong
+
+
+def waits_for(model, state, waits, drained):
+    """Whether something is still under way when all of ``waits``, and that for the products issued (``drained``), have ended, or one of
+    them never does."""
+    wrong, pending, seen = set(), [state], set()
+    while pending:
+        state = pending.pop()
+        if state in seen:
+            continue
+        seen.add(state)
+        following = list(model.events(state))
+        if all(model.passes(state, *wait)[0] for wait in waits) and not (drained and state[3]):
+            if state[2] or state[3]:
+                wrong.add("left")
+            continue
+        if not following:
+            wrong.add("stuck")
+        pending.extend(following)
+    return wrong
+
+
+def started(model, state, warp):
+    """Stages whose copies a warp has started."""
+    program, place = model.programs[warp], state[0][warp]
+    place = place if place >= 0 else ~place
+    return sum(effect[0] == "copy" for step in program[:place] for effect in step[2])
+
+
+def stream(depth, ring):
+    """The warps of a CTA of mxfp4_stream.cu: copies (of the first stages without a wait), exponents, products, read-out."""
+    stages = range(depth)
+    needs = {("sums",): 1, **{(name, s): need for name, need in (("full", 2), ("scales", 1), ("empty", 1)) for s in range(ring)}}
+    copies = [(("empty", i % ring) if i >= ring else None, i // ring - 1, [("arrive", ("full", i % ring)), ("copy", ("full", i % ring), i)]) for i in stages]
+    exponents = [(("empty", i % ring), i // ring - 1, [("arrive", ("scales", i % ring))]) for i in stages]
+    products = [step for i in stages for step in (
+        (("full", i % ring), i // ring, []),
+        (("scales", i % ring), i // ring, [("product", (("empty", i % ring),) + ((("sums",),) if i + 1 == depth else ()))]))]
+    return Model([copies, exponents, products, [(("sums",), 0, [])]], needs)
+
+
+@pytest.mark.parametrize("depth,ring", [(1, 1), (1, 2), (2, 2), (3, 2), (5, 2), (4, 3)])
+def test_streams_wait_for_no_phase_too_early_and_for_none_for_good(depth, ring):
+    assert stream(depth, ring).orders() == set()
+
+
+@pytest.mark.parametrize("depth,ring", [(1, 1), (1, 2), (2, 2), (3, 2), (4, 2), (4, 3)])
+@pytest.mark.parametrize("awaited", [True, False])
+def test_nothing_is_under_way_when_a_stream_has_given_up(depth, ring, awaited):
+    """The copies that the ring can still hold, and the products, are awaited when all warps have ended.  The model sees what is left where the
+    warps that copy and multiply wait at their own end, and only if they know of a failure by then: another may give up after it."""
+    model = stream(depth, ring)
+
+    def leave(state):
+        stages = started(model, state, 0)
+        waits = [(("full", i % ring), i // ring) for i in range(max(0, stages - ring), stages)]
+        return waits_for(model, state, waits if awaited or state[0][0] < 0 else [], awaited or state[0][2] < 0)
+
+    assert model.ways_out(leave) == (set() if awaited else {"left"})
 
 
 def pair(tiles, depth, ring, relayed=True):
