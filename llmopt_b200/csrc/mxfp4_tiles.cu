@@ -44,7 +44,8 @@ constexpr uint32_t kHolder = (5 * kMostStages + 2 * kSums + 1) * 8, kAbort = kHo
 constexpr uint32_t kStaging = kEpilogueWarps * kStagingBytes;
 // Joined tiles of a plan: their number, then first row and expert << 16 | rows of each, in front of the staging.
 constexpr uint32_t kCount = kAbort + 4, kMostJoined = 512, kList = kMostJoined * 8;
-static_assert(kCount + 4 <= kFront && kStaging % 1024 == 0 && kList % 1024 == 0, "alignment of tiles");
+constexpr uint32_t kIssued = kCount + 4;  // stages that either CTA has asked for, where somebody gave up
+static_assert(kIssued + 8 <= kFront && kStaging % 1024 == 0 && kList % 1024 == 0, "alignment of tiles");
 static_assert(kStagingBytes >= 32 * 64, "a box of results");
 
 struct Work {
@@ -55,11 +56,15 @@ struct Work {
   uint32_t list;                       // bytes of the list of joined tiles; 0: the plan's
 };
 
-// The first CTA's barriers, from either.
-__device__ __forceinline__ uint32_t first_address(uint32_t local) {
+// A word or barrier of either CTA, from either; the first one's barriers.
+__device__ __forceinline__ uint32_t pair_address(uint32_t local, uint32_t rank) {
   uint32_t remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(0u));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
   return remote;
+}
+__device__ __forceinline__ uint32_t first_address(uint32_t local) { return pair_address(local, 0u); }
+__device__ __forceinline__ void pair_store(uint32_t local, uint32_t rank, uint32_t value) {
+  asm volatile("st.relaxed.cluster.shared::cluster.b32 [%0], %1;" ::"r"(pair_address(local, rank)), "r"(value) : "memory");
 }
 // The two CTAs hand each other shared memory (exponents laid down, stages read) and tensor memory (sums read out) by barriers whose arrivals and
 // waits have to be of the cluster's scope: one that names none is the CTA's, and orders nothing between threads of two CTAs.  They are relaxed,
@@ -84,6 +89,10 @@ __device__ __forceinline__ bool pair_wait(uint32_t bar, uint32_t parity) {
         : "memory");
   asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
   return __all_sync(0xffffffffu, done != 0u);
+}
+// Bytes that the barrier waits for and nobody will send.
+__device__ __forceinline__ void barrier_forgo(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 // A tile to this CTA's shared memory whose bytes the barrier of the first one counts.
 __device__ __forceinline__ void pair_load(uint32_t destination, const CUtensorMap* map, int32_t x, int32_t y, uint32_t first) {
@@ -215,21 +224,24 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     return {at.x, at.x + (at.y & 0xffffu), (at.y >> 16) * p.n + column, column};
   };
   const uint32_t half_bytes = work.rows / 2u * kRowBytes;
+  auto boxes_of = [&](uint32_t ks) { return min(kBoxes, (p.k - ks * kDepth + kBoxDepth - 1u) / kBoxDepth); };
   // rows that a product takes, half of them from either CTA
   auto width = [&](const Place& at) { return max((at.end - at.row + 31u) / 32u * 32u, 32u); };
-  auto give_up = [&]() {
-    *abort_flag = 1u;
+  auto give_up = [&]() {  // for both CTAs
+    pair_store(base + kAbort, 0u, 1u);
+    pair_store(base + kAbort, 1u, 1u);
     if (error_word) atomicExch(error_word, 1u);
   };
 
+  uint32_t issued = 0;  // stages over all tiles of this pair, by warp 0
   if (warp == 0) {
-    uint32_t issued = 0, s = 0, phase = 1;  // stages over all tiles of this pair
+    uint32_t s = 0, phase = 1;
     bool ok = true;
     for (uint32_t tile = pair; tile < tiles && ok; tile += pairs) {
       const Place at = place(tile);
       const uint32_t x_row = uniform(at.row + rank * (width(at) / 2u)), w_row = uniform(at.w_row) + rank * kColumns;
       for (uint32_t ks = 0; ks < k_stages; ++ks, ++issued) {
-        const uint32_t stage = base + work.ring + s * work.stage_bytes, boxes = min(kBoxes, (p.k - ks * kDepth + kBoxDepth - 1u) / kBoxDepth);
+        const uint32_t stage = base + work.ring + s * work.stage_bytes, boxes = boxes_of(ks);
         ok = !*abort_flag && pair_wait(empty + s * 8, phase);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) {
@@ -250,14 +262,6 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         if (++s == work.stages) s = 0, phase ^= 1u;
       }
     }
-    // on the way out after a failure the copies already started must land first: both CTAs' have when the first one's barriers say so
-    if (rank == 0u && (!ok || *abort_flag))
-      for (uint32_t i = issued > work.stages ? issued - work.stages : 0u; i < issued; ++i)
-        barrier_wait(full + (i % work.stages) * 8, (i / work.stages) & 1u);
-    // but for a stage that only the second one came to ask for, which nothing counts any more: it has a millisecond to land
-    if (rank == 1u && (!ok || *abort_flag))
-      for (uint32_t i = 0; i < 1000u; ++i) __nanosleep(1000);
-    __syncwarp();
   } else if (warp == 1 && rank == 1u) {
     // the first CTA issues for both, and hears from here that exponents lie in the second one's memory
     uint32_t s = 0, phase = 0;
@@ -316,14 +320,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         if (++s == work.stages) s = 0, phase ^= 1u;
       }
     }
-    if (!ok) {
-      // the products already issued read both CTAs' memory
-      give_up();
-      if (elect_one())
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drained) : "memory");
-      __syncwarp();
-      pair_wait(drained, 0u);
-    }
+    if (!ok) give_up();
   } else if (warp < 2u + kScaleWarps) {
     // the words of group warp - 2 of a stage, of the CTA's weight rows and of the tile's rows of x: lane, lane + 32, ...
     const uint32_t group = warp - 2u, words = words_of(p.k), last_mask = last_word_mask(p.k);
@@ -435,6 +432,32 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 
   __syncthreads();
   cluster_sync();  // neither CTA leaves, or gives its tensor memory back, while the other's products or arrivals reach it
+  // Whoever gave up has said so to both by now.  What was started then must end before the pair leaves: products, and the copies of both, which
+  // the first one's barriers count and of which those that nobody waited for are among the ring's last.  Of a stage that one CTA alone
+  // came to ask for they would wait for the other's share too.
+  if (*abort_flag) {
+    if (threadIdx.x == 0) pair_store(base + kIssued + rank * 4u, 0u, issued);
+    __syncwarp();
+    cluster_sync();
+    if (rank == 0u && warp == 0) {
+      const volatile uint32_t* const of = reinterpret_cast<const volatile uint32_t*>(base_pointer + kIssued);
+      const uint32_t first = of[0], second = of[1], last = max(first, second);
+      for (uint32_t i = last > work.stages ? last - work.stages : 0u; i < last; ++i) {
+        const uint32_t bar = full + (i % work.stages) * 8, bytes = boxes_of(i % k_stages) * (kBoxBytes + half_bytes);
+        if (lane == 0 && i >= first) barrier_expect_tx(bar, bytes);
+        if (lane == 0 && i >= second) barrier_forgo(bar, bytes);
+        __syncwarp();
+        barrier_wait(bar, (i / work.stages) & 1u);
+      }
+    } else if (rank == 0u && warp == 1) {
+      if (elect_one())
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drained) : "memory");
+      __syncwarp();
+      pair_wait(drained, 0u);
+    }
+    __syncwarp();
+    cluster_sync();
+  }
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemColumns) : "memory");

@@ -202,6 +202,33 @@ def test_pairs_wait_for_no_phase_too_early_and_for_none_for_good(tiles, depth, r
     assert pair(tiles, depth, ring).orders() == set()
 
 
+@pytest.mark.parametrize("tiles,depth,ring", [(1, 1, 2), (1, 2, 1), (1, 2, 2), (2, 1, 2)])
+@pytest.mark.parametrize("awaited", [True, False])
+def test_nothing_is_under_way_when_a_pair_has_given_up(tiles, depth, ring, awaited):
+    """The first CTA waits for the copies of both, and makes up for what a stage lacks that one of them alone came to ask for.  The model sees
+    what is left or waited for in vain where the warps that copy and multiply wait at their own end, only if they know of a failure by
+    then, and for the stages that the first CTA asked for."""
+    model = pair(tiles, depth, ring)
+
+    def leave(state):
+        first, second = started(model, state, 0), started(model, state, 3)
+        places, counts, copies, products = state
+        if not awaited:
+            waits = [(("full", i % ring), i // ring) for i in range(max(0, first - ring), first)]
+            return waits_for(model, state, waits if places[0] < 0 else [], places[-1] < 0)
+        last = max(first, second)
+        for i in range(max(0, last - ring), last):
+            if i >= first:  # its own word, and its half of the bytes, which it does not count
+                counts = model.arrive(model.arrive(counts, ("full", i % ring)), ("full", i % ring))
+            if i >= second:
+                counts = model.arrive(counts, ("full", i % ring))
+        waits = [(("full", i % ring), i // ring) for i in range(max(0, last - ring), last)]
+        return waits_for(model, (places, counts, copies, products), waits, True)
+
+    wrong = model.ways_out(leave)
+    assert wrong == set() if awaited else wrong & {"left", "stuck"}
+
+
 def test_the_model_sees_exponents_that_do_not_wait():
     assert pair(1, 3, 2, relayed=False).orders() & {"early", "stuck"}
 
