@@ -1,0 +1,40 @@
+"""Calls of the MXFP4 operators at the ends of what they take: gates far from zero, sizes, raw pointers, streams, failures."""
+
+import numpy as np
+import pytest
+
+import mxfp4_oracle as mx
+from test_gpu_mxfp4 import HALF_STEP, blank, check, context, device, from_bits, read, upload
+
+pytestmark = pytest.mark.gpu
+
+
+# slots and k: a tile's CTA by itself, a cluster that shares out k, pairs of CTAs with the plan's tiles and with joined ones
+@pytest.mark.parametrize("slots,k", [(40, 64), (40, 4096), (200, 64), (200, 2048)])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_pairs_with_gates_far_from_zero(runtime, dtype, slots, k):
+    """silu of a gate near -88 is near 2^-120, which the other column can bring back into the range of 16 bits: the score is the gate, the
+    other column a power of two times it.  In steps of 2^-23: e^(gate / 3) is off by 2 (ex2.approx) and by what its argument is, whose factor
+    and product round to 1.5 of 2^-24 of gate / 3; it enters three times.  The reciprocal is off by 1, eight other operations by a half each."""
+    from llmopt_b200 import dispatch
+
+    power = 120 if dtype == "float16" else 100
+    score = np.linspace(80.0, 103.0 if dtype == "float16" else 150.0, slots).astype(np.float32)
+    if dtype == "bfloat16":
+        score[::5] *= -1  # gates above zero
+    n = 34
+    x, w = (np.zeros((slots, k), np.uint8), np.full((slots, k // 32), 127, np.uint8)), (np.zeros((n, k), np.uint8), np.full((n, k // 32), 127, np.uint8))
+    x[0][:, k - 40] = 2
+    w[0][0::2, k - 40], w[0][1::2, k - 40], w[1][1::2, (k - 40) // 32] = 10, 2, 127 + power  # -1, 2^power
+    gate, up = -score.astype(np.float64), score.astype(np.float64) * 2.0 ** power
+    want = np.repeat((gate / (1 + np.exp(-gate)) * up)[:, None], n // 2, 1)
+    xt, wt = upload(runtime, x), upload(runtime, w)
+    y = blank(runtime, (slots, n // 2), dtype, 256)
+    dispatch.dispatch_mxfp4_expert_rows(context(runtime), input=xt[0], input_scales=xt[1], weight=wt[0], weight_scales=wt[1], experts=1,
+                                        plan=device(runtime, mx.plan_of(np.zeros(slots, int), 1)).buffer, output=y, score_of_slot=device(runtime, score))
+    steps = 3 * (2 + 0.75 * np.abs(gate) / 3) + 1 + 8 / 2
+    limit = np.abs(want) * (HALF_STEP[dtype] * (1 + 2.0 ** -10) + steps[:, None] * 2.0 ** -23) + (2.0 ** -25 if dtype == "float16" else 0.0)
+    got = from_bits(read(y, 256), dtype)
+    beyond = np.abs(want) - limit > (65520.0 if dtype == "float16" else np.inf)  # from there on the nearest of f16 is infinity
+    assert (got[beyond] == -np.inf).all() and beyond.mean() < 0.1
+    check(got[~beyond], want[~beyond], limit[~beyond])
