@@ -406,7 +406,7 @@ def dispatch_mxfp4_linear(context: Context, *, input: Tensor, input_scales: Tens
     buffers = [input.buffer, input_scales.buffer, weight.buffer, weight_scales.buffer, (output if bias is None else bias).buffer,
                output.buffer]
     return [_run(context, f"llmopt_mxfp4_linear_{element}", buffers,
-                 parameters.mxfp4_linear(m=m, n=n, k=k, has_bias=bias is not None), (linear_f16_grid(m * n), 1, 1))]
+                 parameters.mxfp4_linear(m=m, n=n, k=k, has_bias=bias is not None), (1, 1, 1))]
 
 
 def dispatch_mxfp4_expert_rows(context: Context, *, input: Tensor, input_scales: Tensor, weight: Tensor, weight_scales: Tensor,
