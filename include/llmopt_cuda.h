@@ -299,7 +299,7 @@ int llmopt_cuda_mxfp4_linear(llmopt_cuda_context* context, int type, const void*
                              int64_t k, void* stream);
 /* Rows sorted by expert (slots of them, as llmopt_route_plan sorts and lists them) times their experts' n rows of w
  * [experts * n, k].  paired: neighbouring columns are a gate and a value, out [slots, n / 2] in `type` (f16 or bf16) =
- * silu(score * gate) * (score * value); otherwise out is f32 [slots, n] and score_of_slot is not read. */
+ * silu(score * gate) * (score * value); otherwise out is f32 [slots, n], whatever `type`, and score_of_slot is not read. */
 int llmopt_cuda_mxfp4_expert_rows(llmopt_cuda_context* context, int type, const void* x_codes, const void* x_scales,
                                   const void* w_codes, const void* w_scales, const void* plan, const void* score_of_slot,
                                   void* out, int64_t slots, int64_t n, int64_t k, int64_t experts, int paired, void* stream);

@@ -1727,6 +1727,7 @@ int llmopt_cuda_mxfp4_expert_rows(llmopt_cuda_context* context, int type, const 
   launch.operand(score_of_slot, paired ? mxfp4_extent(slots, 4) : 0);
   launch.operand(out, paired ? mxfp4_extent(slots, n / 2) * mxfp4_size(type) : mxfp4_extent(slots, n) * 4);
   launch.sizes({slots, n, k, experts, paired != 0});
+  if (!paired && type == LLMOPT_CUDA_F32) type = LLMOPT_CUDA_BF16;  // rows in fp32 are the same in either form
   return launch.run(std::string("llmopt_mxfp4_expert_rows") + mxfp4_suffix(type));
 }
 

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import mxfp4_oracle as mx
-from test_gpu_mxfp4 import HALF_STEP, blank, check, context, device, from_bits, read, upload
+from test_gpu_mxfp4 import HALF_STEP, allowed, blank, check, context, device, expert_case, from_bits, read, upload
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +38,29 @@ def test_pairs_with_gates_far_from_zero(runtime, dtype, slots, k):
     beyond = np.abs(want) - limit > (65520.0 if dtype == "float16" else np.inf)  # from there on the nearest of f16 is infinity
     assert (got[beyond] == -np.inf).all() and beyond.mean() < 0.1
     check(got[~beyond], want[~beyond], limit[~beyond])
+
+
+# ---- raw pointers -----------------------------------------------------------------------------------------
+
+def on_gpu(array):
+    import torch
+
+    array = np.ascontiguousarray(array)
+    return torch.from_numpy(array.view(np.int32) if array.dtype == np.uint32 else array).cuda()
+
+
+@pytest.mark.parametrize("element", ["f32", "f16", "bf16"])
+def test_sums_of_expert_rows_are_fp32_whatever_the_type(runtime, element):
+    import torch
+
+    rng = np.random.default_rng(41)
+    counts, n, k = [5, 0, 2], 66, 96
+    expert_of_slot, x, w, _ = expert_case(rng, counts, n, k)
+    xv, wv = mx.values(*x), mx.values(*w).reshape(len(counts), n, k)
+    held = [on_gpu(a) for a in (mx.pack(x[0]), mx.words(x[1]), mx.pack(w[0]), mx.words(w[1]), mx.plan_of(expert_of_slot, len(counts)))]
+    y = torch.full((7, n), float("nan"), device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    runtime.mxfp4_expert_rows_pointers(element, *[t.data_ptr() for t in held], None, y.data_ptr(), 7, n, k, len(counts), False, stream)
+    want = np.einsum("sk,snk->sn", xv, wv[expert_of_slot])
+    limit = np.stack([allowed(xv[i:i + 1], wv[e], want[i:i + 1], "float32")[0] for i, e in enumerate(expert_of_slot)])
+    check(y.cpu().double().numpy(), want, limit)
