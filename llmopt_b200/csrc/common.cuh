@@ -131,9 +131,15 @@ inline void launch_cluster_kernel(const KernelArgs& launch, void (*kernel)(Param
   cudaLaunchKernelEx(&config, kernel, static_cast<Args&&>(args)...);
 }
 
+// A launcher's other answer beside fail's: the arguments are in order, and CUDA refused what the launch needs.
+constexpr int kLaunchFailed = 2;
+inline int fail_launch(const KernelArgs& args, const std::string& message) {
+  fail(args, message);
+  return kLaunchFailed;
+}
 inline int check_launch(const KernelArgs& args) {
   cudaError_t status = cudaGetLastError();
-  if (status != cudaSuccess) return fail(args, std::string("launch failed: ") + cudaGetErrorString(status));
+  if (status != cudaSuccess) return fail_launch(args, std::string("launch failed: ") + cudaGetErrorString(status));
   return 0;
 }
 

@@ -323,9 +323,9 @@ int run(const KernelArgs& args, const Problem& p, uint32_t row_tiles) {
   work.share = (rows + work.splits - 1u) / work.splits;
   while (shared_bytes<NT>(work) > kMostShared) --work.stages;
   auto kernel = stream_kernel<NT, S>;
-  LLMOPT_REQUIRE((allow_shared<stream_kernel<NT, S>, kMostShared>()), "shared memory request was refused");
+  if (!allow_shared<stream_kernel<NT, S>, kMostShared>()) return fail_launch(args, "shared memory request was refused");
   CUtensorMap map_w, map_x;
-  LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.box_rows), "tensor map was refused");
+  if (!make_map(&map_w, p.w, p.k, p.w_rows, kColumns) || !make_map(&map_x, p.x, p.k, p.m, work.box_rows)) return fail_launch(args, "tensor map was refused");
   const dim3 grid((uint32_t)tiles * work.splits);
   if (work.splits == 1u)
     launch_kernel(args, kernel, grid, dim3(kThreads), shared_bytes<NT>(work), map_w, map_x, p, work, context_device_error(args.ctx));

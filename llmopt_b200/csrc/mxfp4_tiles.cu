@@ -494,9 +494,9 @@ int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
   work.ring = kFront + work.list + (tiles > pairs ? kStaging : 0u);
   work.stages = (kMostShared - 1024u - work.ring) / work.stage_bytes;
   if (work.stages > kMostStages) work.stages = kMostStages;
-  LLMOPT_REQUIRE((allow_shared<tiles_kernel<S>, kMostShared>()), "shared memory request was refused");
+  if (!allow_shared<tiles_kernel<S>, kMostShared>()) return fail_launch(args, "shared memory request was refused");
   CUtensorMap map_w, map_x;
-  LLMOPT_REQUIRE(make_map(&map_w, p.w, p.k, p.w_rows, kColumns) && make_map(&map_x, p.x, p.k, p.m, work.rows / 2u), "tensor map was refused");
+  if (!make_map(&map_w, p.w, p.k, p.w_rows, kColumns) || !make_map(&map_x, p.x, p.k, p.m, work.rows / 2u)) return fail_launch(args, "tensor map was refused");
   CUtensorMap map_out = map_x;  // not read without boxes
   const uint32_t columns = kPaired<S> ? p.n / 2u : p.n;
   if (S != kStoreFloat && columns % 8u == 0 && ((uintptr_t)p.out & 15u) == 0) {

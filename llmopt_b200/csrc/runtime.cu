@@ -1658,7 +1658,7 @@ struct PointerLaunch {
     if (current != args.ctx->device) CUDA_TRY(cudaSetDevice(args.ctx->device), "cudaSetDevice failed");
     const int status = found->launcher(args);
     if (current != args.ctx->device) cudaSetDevice(current);
-    if (status != 0) return set_error(LLMOPT_CUDA_INVALID_ARGUMENT, message);
+    if (status != 0) return set_error(status == kLaunchFailed ? LLMOPT_CUDA_FAILURE : LLMOPT_CUDA_INVALID_ARGUMENT, message);
     return LLMOPT_CUDA_OK;
   }
 };

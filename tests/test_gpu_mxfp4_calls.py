@@ -64,3 +64,40 @@ def test_sums_of_expert_rows_are_fp32_whatever_the_type(runtime, element):
     want = np.einsum("sk,snk->sn", xv, wv[expert_of_slot])
     limit = np.stack([allowed(xv[i:i + 1], wv[e], want[i:i + 1], "float32")[0] for i, e in enumerate(expert_of_slot)])
     check(y.cpu().double().numpy(), want, limit)
+
+
+def cudart():
+    """The CUDA runtime that torch has loaded."""
+    import ctypes
+
+    with open("/proc/self/maps") as maps:
+        return ctypes.CDLL(next(line.split()[-1] for line in maps if "libcudart" in line))
+
+
+def test_a_launch_that_cuda_refuses_is_no_invalid_argument(runtime):
+    """The stream's capture has been spoilt by a wait, so nothing can be launched on it until the capture has ended."""
+    import ctypes
+
+    import torch
+
+    from llmopt_b200.cuda_native import NativeError
+
+    torch.cuda.init()
+    x, codes, scales = torch.ones(3, 64, device="cuda"), torch.zeros(3, 32, dtype=torch.uint8, device="cuda"), torch.zeros(1, 3, dtype=torch.int32, device="cuda")
+    y = torch.zeros(3, 3, device="cuda")
+    torch.cuda.synchronize()
+    stream, graph, lib = torch.cuda.Stream(), ctypes.c_void_p(), cudart()
+    quantize = lambda: runtime.mxfp4_quantize_pointers("f32", x.data_ptr(), None, codes.data_ptr(), scales.data_ptr(), 3, 3, 64, 64, stream.cuda_stream)
+    operand = codes.data_ptr(), scales.data_ptr()
+    product = lambda: runtime.mxfp4_linear_pointers("f32", *operand, *operand, None, y.data_ptr(), 3, 3, 64, stream.cuda_stream)
+    assert lib.cudaStreamBeginCapture(ctypes.c_void_p(stream.cuda_stream), 2) == 0
+    assert lib.cudaStreamSynchronize(ctypes.c_void_p(stream.cuda_stream)) != 0
+    for call in (quantize, product):
+        with pytest.raises(NativeError, match="launch failed"):
+            call()
+    assert lib.cudaStreamEndCapture(ctypes.c_void_p(stream.cuda_stream), ctypes.byref(graph)) != 0
+    lib.cudaGetLastError()
+    quantize()
+    product()
+    stream.synchronize()
+    assert (y == 64.0).all()  # ones in four bits are ones
