@@ -279,7 +279,8 @@ int llmopt_cuda_w4a16_linear(llmopt_cuda_context* context, const void* input, co
  * k is a multiple of 32.  The kernels of the same names (llmopt_mxfp4_quantize_f16 and so on) do the same for buffers in
  * batches and plans; these run one of them on `stream` (a cudaStream_t; NULL = the default stream) of the context's device without
  * waiting, keep nothing between calls and use no memory but the operands, so calls on different streams may overlap and a stream capture
- * may hold them.  A wait inside a kernel that runs out is reported by the context's next wait.  `type`: what the operand without codes
+ * may hold them; what the context's own stream still has to do (a buffer's write, a batch) is not waited for.  Waits inside the kernels are
+ * bounded; one that runs out is reported by llmopt_cuda_mxfp4_synchronize and by no other wait.  `type`: what the operand without codes
  * is held in. */
 #define LLMOPT_CUDA_F16 0
 #define LLMOPT_CUDA_BF16 1
@@ -303,6 +304,10 @@ int llmopt_cuda_mxfp4_linear(llmopt_cuda_context* context, int type, const void*
 int llmopt_cuda_mxfp4_expert_rows(llmopt_cuda_context* context, int type, const void* x_codes, const void* x_scales,
                                   const void* w_codes, const void* w_scales, const void* plan, const void* score_of_slot,
                                   void* out, int64_t slots, int64_t n, int64_t k, int64_t experts, int paired, void* stream);
+/* Waits for `stream` (NULL = the default stream) and fails if a wait inside a kernel of the calls above on this context has run out, on
+ * whatever stream: which call's is not known, so none of the results since the last clear are to be used, and everybody who asks is
+ * told until one call says clear != 0 (which is told too; none of the calls may be under way then). */
+int llmopt_cuda_mxfp4_synchronize(llmopt_cuda_context* context, void* stream, int clear);
 
 /* ---- entry point that allocates nothing ---------------------------------------------- */
 

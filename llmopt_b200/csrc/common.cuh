@@ -48,6 +48,7 @@ struct KernelArgs {
   const struct RotaryPackFusion* rotary_fusion;
   bool in_plan;  // captured into a plan, which replays it
   bool apart;  // this launch starts when its predecessor has ended, also where overlap is allowed
+  uint32_t* error_word;  // where kernels say that a wait ran out; null: the context's, which its own waits read
 };
 
 // Bytes between the sequences of a batched short-conv step.

@@ -40,6 +40,7 @@ struct Shape {
 struct Work {
   uint32_t row_tiles, column_tiles, splits, stages, box_rows;
   uint32_t share;  // rows that a CTA of a cluster joins
+  uint32_t wait_limit;  // how often a wait looks; 0: all give up at once
 };
 // Shared memory, 1024 of it for the alignment of the ring; behind the barriers the sums of a cluster's CTAs, [from][row of the share][column],
 // and a row that may be read but not used.
@@ -85,7 +86,7 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
       }
       barrier_init(sums_full, 1);  // one tcgen05.commit
       barrier_init(drained, 1);    // the same, where somebody gave up
-      *abort_flag = 0u;
+      *abort_flag = work.wait_limit == 0u;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
@@ -151,11 +152,12 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
   const uint32_t tmem_base = warp > 0 ? uniform(*holder) : 0u;
 
   uint32_t issued = min(work.stages, stage1 - stage0);  // stages, by warp 0
+  bool multiplied = false;                              // by warp 1
   if (warp == 0) {
     bool ok = true;
     uint32_t s = 0, phase = 0;
     for (uint32_t ks = stage0 + issued; ks < stage1; ++ks, ++issued) {
-      ok = !*abort_flag && warp_wait(empty + s * 8, phase);
+      ok = !*abort_flag && warp_wait(empty + s * 8, phase, work.wait_limit);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
         give_up();
@@ -171,9 +173,10 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     uint32_t s = 0, phase = 0;
     for (uint32_t ks = stage0; ks < stage1; ++ks) {
       const uint32_t stage = base + s * Z::kStageBytes;
-      ok = !*abort_flag && warp_wait(full + s * 8, phase) && warp_wait(scales_full + s * 8, phase);
+      ok = !*abort_flag && warp_wait(full + s * 8, phase, work.wait_limit) && warp_wait(scales_full + s * 8, phase, work.wait_limit);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
+      multiplied = true;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t scales = tmem_base + NT + (ks & 1u) * Z::kScaleColumns, x_scales = scales + kStageWords * 4u, left = p.k - ks * kDepth;
       const uint64_t a = operand_descriptor(stage), b = operand_descriptor(stage + Z::kWeightBytes);
@@ -207,7 +210,7 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
       for (uint32_t a = 0; a < kAhead; ++a) {
         const uint32_t ks = first + a;
         if (ks >= stage1 || !ok) break;
-        ok = !*abort_flag && warp_wait(empty + s * 8, phase);
+        ok = !*abort_flag && warp_wait(empty + s * 8, phase, work.wait_limit);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint32_t mask = ks * kStageWords + group + 1u == words ? last_mask : 0xffffffffu;
@@ -228,7 +231,7 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     const uint32_t quarter = warp & 3u;
     float own = splits == 1u ? piece_operand<S>(p, at.row, at.end, at.column + quarter * 32u) : 0.0f;
     if (ok) {
-      ok = !*abort_flag && warp_wait(sums_full, 0u);
+      ok = !*abort_flag && warp_wait(sums_full, 0u, work.wait_limit);
       ok = __all_sync(0xffffffffu, ok);
     }
     if (splits > 1u) cluster_wait();
@@ -272,7 +275,7 @@ stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__
     if (warp == 0) {
       for (uint32_t i = issued > work.stages ? issued - work.stages : 0u; i < issued; ++i)
         barrier_wait(full + (i % work.stages) * 8, (i / work.stages) & 1u);
-    } else if (warp == 1) {
+    } else if (multiplied) {
       if (elect_one()) mma_commit(drained);
       __syncwarp();
       warp_wait(drained, 0u);
@@ -308,7 +311,7 @@ template <uint32_t NT, Store S>
 int run(const KernelArgs& args, const Problem& p, uint32_t row_tiles) {
   using Z = Shape<NT>;
   const uint32_t sms = (uint32_t)context_sm_count(args.ctx), k_stages = (p.k + kDepth - 1u) / kDepth;
-  Work work = {row_tiles, (p.n + kColumns - 1u) / kColumns, 1u, 0u, p.plan.tiles ? 16u : NT, 0u};
+  Work work = {row_tiles, (p.n + kColumns - 1u) / kColumns, 1u, 0u, p.plan.tiles ? 16u : NT, 0u, context_mxfp4_wait_limit(args.ctx)};
   const size_t tiles = (size_t)work.row_tiles * work.column_tiles;
   LLMOPT_REQUIRE(tiles < (1u << 28), "too many tiles");
   // CTAs that share a tile's k while tiles leave SMs without work; powers of two, which leave the fewest SMs of a GPC over.  us with 1, 2, 4, 8
@@ -328,10 +331,10 @@ int run(const KernelArgs& args, const Problem& p, uint32_t row_tiles) {
   if (!make_map(&map_w, p.w, p.k, p.w_rows, kColumns) || !make_map(&map_x, p.x, p.k, p.m, work.box_rows)) return fail_launch(args, "tensor map was refused");
   const dim3 grid((uint32_t)tiles * work.splits);
   if (work.splits == 1u)
-    launch_kernel(args, kernel, grid, dim3(kThreads), shared_bytes<NT>(work), map_w, map_x, p, work, context_device_error(args.ctx));
+    launch_kernel(args, kernel, grid, dim3(kThreads), shared_bytes<NT>(work), map_w, map_x, p, work, error_word_of(args));
   else
     launch_cluster_kernel(args, kernel, grid, dim3(kThreads), shared_bytes<NT>(work), work.splits, map_w, map_x, p, work,
-                          context_device_error(args.ctx));
+                          error_word_of(args));
   return check_launch(args);
 }
 

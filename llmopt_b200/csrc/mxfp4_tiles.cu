@@ -54,6 +54,7 @@ struct Work {
   uint32_t stages, stage_bytes, ring;  // of shared memory; where the ring begins
   uint32_t boxes;                      // results leave in boxes
   uint32_t list;                       // bytes of the list of joined tiles; 0: the plan's
+  uint32_t wait_limit;                 // how often a wait looks; 0: all give up at once
 };
 
 // A word or barrier of either CTA, from either; the first one's barriers.
@@ -77,9 +78,9 @@ __device__ __forceinline__ void shared_release() { asm volatile("fence.release.s
 __device__ __forceinline__ void first_arrive(uint32_t first) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(first) : "memory");
 }
-__device__ __forceinline__ bool pair_wait(uint32_t bar, uint32_t parity) {
-  uint32_t done = 0;
-  for (uint32_t spin = 0; spin < kWaitLimit && !done; ++spin)
+__device__ __forceinline__ bool pair_wait(uint32_t bar, uint32_t parity, uint32_t limit = kWaitLimit) {
+  uint32_t done = 0, looks = 0;
+  do {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
@@ -87,6 +88,7 @@ __device__ __forceinline__ bool pair_wait(uint32_t bar, uint32_t parity) {
         : "=r"(done)
         : "r"(bar), "r"(parity)
         : "memory");
+  } while (!done && ++looks < limit);
   asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
   return __all_sync(0xffffffffu, done != 0u);
 }
@@ -186,7 +188,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       barrier_init(sums_empty + s * 8, 2 * kEpilogueWarps);
     }
     barrier_init(drained, 1);
-    *abort_flag = 0u;
+    *abort_flag = work.wait_limit == 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncwarp();
@@ -233,7 +235,8 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     if (error_word) atomicExch(error_word, 1u);
   };
 
-  uint32_t issued = 0;  // stages over all tiles of this pair, by warp 0
+  uint32_t issued = 0;      // stages over all tiles of this pair, by warp 0
+  bool multiplied = false;  // by warp 1 of the first CTA
   if (warp == 0) {
     uint32_t s = 0, phase = 1;
     bool ok = true;
@@ -242,7 +245,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       const uint32_t x_row = uniform(at.row + rank * (width(at) / 2u)), w_row = uniform(at.w_row) + rank * kColumns;
       for (uint32_t ks = 0; ks < k_stages; ++ks, ++issued) {
         const uint32_t stage = base + work.ring + s * work.stage_bytes, boxes = boxes_of(ks);
-        ok = !*abort_flag && pair_wait(empty + s * 8, phase);
+        ok = !*abort_flag && pair_wait(empty + s * 8, phase, work.wait_limit);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) {
           give_up();
@@ -268,7 +271,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
     bool ok = true;
     for (uint32_t tile = pair; tile < tiles && ok; tile += pairs)
       for (uint32_t ks = 0; ks < k_stages; ++ks) {
-        ok = !*abort_flag && warp_wait(laid + s * 8, phase);
+        ok = !*abort_flag && warp_wait(laid + s * 8, phase, work.wait_limit);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (lane == 0) {
@@ -286,14 +289,15 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       const uint32_t rows = uniform(width(place(tile)));
       const uint32_t low = mxf4_instruction(2u * kColumns, rows, 0u), high = mxf4_instruction(2u * kColumns, rows, 1u);
       const uint32_t which = turn % kSums, sums = tmem_base + which * kMostRows, scales = tmem_base + kSums * kMostRows;
-      ok = !*abort_flag && pair_wait(sums_empty + which * 8, ((turn / kSums) & 1u) ^ 1u);
+      ok = !*abort_flag && pair_wait(sums_empty + which * 8, ((turn / kSums) & 1u) ^ 1u, work.wait_limit);
       ok = __all_sync(0xffffffffu, ok);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       for (uint32_t ks = 0; ks < k_stages && ok; ++ks) {
         const uint32_t stage = base + work.ring + s * work.stage_bytes;
-        ok = !*abort_flag && pair_wait(full + s * 8, phase) && pair_wait(scales_full + s * 8, phase);
+        ok = !*abort_flag && pair_wait(full + s * 8, phase, work.wait_limit) && pair_wait(scales_full + s * 8, phase, work.wait_limit);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
+        multiplied = true;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t left = p.k - ks * kDepth;
         const uint64_t a = operand_descriptor(stage), b = operand_descriptor(stage + kInputAt);
@@ -360,7 +364,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
 #pragma unroll
       for (uint32_t a = 0; a < kAhead; ++a) {
         if (first + a >= all || !ok) break;
-        ok = !*abort_flag && warp_wait(vacant + s * 8, phase);
+        ok = !*abort_flag && warp_wait(vacant + s * 8, phase, work.wait_limit);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const uint32_t mask = ks * kStageWords + group + 1u == words ? last_mask : 0xffffffffu;
@@ -391,7 +395,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
       const Place at = place(tile);
       const uint32_t column = at.column + rank * kColumns + quarter * 32u;
       float own = piece_operand<S>(p, at.row + side * 32u, at.end, column);
-      ok = !*abort_flag && pair_wait(sums_full + which * 8, (turn / kSums) & 1u);
+      ok = !*abort_flag && pair_wait(sums_full + which * 8, (turn / kSums) & 1u, work.wait_limit);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) {
         give_up();
@@ -449,7 +453,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ 
         __syncwarp();
         barrier_wait(bar, (i / work.stages) & 1u);
       }
-    } else if (rank == 0u && warp == 1) {
+    } else if (multiplied) {
       if (elect_one())
         asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drained) : "memory");
       __syncwarp();
@@ -471,7 +475,7 @@ namespace mxfp4 {
 template <Store S>
 int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
   const uint32_t pairs = (uint32_t)context_sm_count(args.ctx) / 2u, k_stages = (p.k + kDepth - 1u) / kDepth;
-  Work work = {plan_tiles, (p.n + 2u * kColumns - 1u) / (2u * kColumns), kExpertTile, 0u, 0u, 0u, 0u, 0u};
+  Work work = {plan_tiles, (p.n + 2u * kColumns - 1u) / (2u * kColumns), kExpertTile, 0u, 0u, 0u, 0u, 0u, context_mxfp4_wait_limit(args.ctx)};
   if (!p.plan.tiles) {
     // the height with the shortest estimate: rounds of tiles times the cycles of one, of which a stage takes about 500 and four per row
     uint64_t least = ~0ull;
@@ -506,7 +510,7 @@ int run_tiles(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
   }
   const uint32_t shared = 1024u + work.ring + work.stages * work.stage_bytes;  // 1024 for the alignment of the ring
   launch_cluster_kernel(args, tiles_kernel<S>, dim3(2u * (tiles < pairs ? (uint32_t)tiles : pairs)), dim3(kThreads), shared, 2u, map_w, map_x,
-                        map_out, p, work, context_device_error(args.ctx));
+                        map_out, p, work, error_word_of(args));
   return check_launch(args);
 }
 

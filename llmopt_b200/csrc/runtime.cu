@@ -119,6 +119,9 @@ struct Context {
   // Pinned, device-visible word: kernels whose bounded waits ran out set it; the host
   // reads it after every stream wait.
   uint32_t* device_error = nullptr;
+  // Its neighbour, for calls on raw pointers, which run on streams that the context does not wait for.
+  uint32_t* pointer_error() const { return device_error + 1; }
+  uint32_t mxfp4_wait_limit = 1u << 20;  // how often a wait inside the MXFP4 products looks before it gives up
   // Launches may overlap the tail of their predecessor (programmatic dependent launch).
   bool overlap = true;
   // Expression epilogues registered by digest name (llmopt_cuda_register_expr_epilogue).
@@ -234,6 +237,7 @@ const ExprProgram* context_expr_program(Context* context, const char* name) {
 int context_sm_count(Context* context) { return context->sm_count; }
 bool context_overlap(Context* context) { return context != nullptr && context->overlap; }
 uint32_t* context_device_error(Context* context) { return context->device_error; }
+uint32_t context_mxfp4_wait_limit(Context* context) { return context->mxfp4_wait_limit; }
 
 static void register_kernels(llmopt_cuda_library* library) {
   auto add = [&](const char* name, Launcher launcher) {
@@ -798,6 +802,7 @@ int llmopt_cuda_create_context(int device, llmopt_cuda_context** out) {
   context->device = device;
   context->sm_count = properties.multiProcessorCount;
   if (const char* overlap = getenv("LLMOPT_CUDA_OVERLAP")) context->overlap = overlap[0] != '0';
+  if (const char* limit = getenv("LLMOPT_CUDA_MXFP4_WAIT_LIMIT")) context->mxfp4_wait_limit = (uint32_t)strtoul(limit, nullptr, 10);
   context->name = properties.name;
   status = cudaStreamCreateWithFlags(&context->stream, cudaStreamNonBlocking);
   if (status != cudaSuccess) {
@@ -805,8 +810,8 @@ int llmopt_cuda_create_context(int device, llmopt_cuda_context** out) {
     return cuda_failure("cudaStreamCreate failed", status);
   }
   status = cudaMalloc((void**)&context->argmax_result, sizeof(int));
-  if (status == cudaSuccess) status = cudaHostAlloc((void**)&context->device_error, sizeof(uint32_t), cudaHostAllocMapped);
-  if (status == cudaSuccess) *context->device_error = 0;
+  if (status == cudaSuccess) status = cudaHostAlloc((void**)&context->device_error, 2 * sizeof(uint32_t), cudaHostAllocMapped);
+  if (status == cudaSuccess) context->device_error[0] = context->device_error[1] = 0;
   if (status != cudaSuccess) {
     release(context);
     return cuda_failure("context allocation failed", status);
@@ -1630,6 +1635,7 @@ struct PointerLaunch {
     args.stream = (cudaStream_t)stream;
     args.params = (const uint8_t*)params;
     args.error = &message;
+    args.error_word = context->pointer_error();
   }
   void operand(const void* pointer, size_t bytes) {
     null_pointer |= pointer == nullptr && bytes > 0;
@@ -1729,6 +1735,20 @@ int llmopt_cuda_mxfp4_expert_rows(llmopt_cuda_context* context, int type, const 
   launch.sizes({slots, n, k, experts, paired != 0});
   if (!paired && type == LLMOPT_CUDA_F32) type = LLMOPT_CUDA_BF16;  // rows in fp32 are the same in either form
   return launch.run(std::string("llmopt_mxfp4_expert_rows") + mxfp4_suffix(type));
+}
+
+int llmopt_cuda_mxfp4_synchronize(llmopt_cuda_context* context, void* stream, int clear) {
+  if (context == nullptr) return set_error(LLMOPT_CUDA_FAILURE, "CUDA context has been finalized");
+  int current = -1;
+  CUDA_TRY(cudaGetDevice(&current), "cudaGetDevice failed");
+  if (current != context->device) CUDA_TRY(cudaSetDevice(context->device), "cudaSetDevice failed");
+  const cudaError_t status = cudaStreamSynchronize((cudaStream_t)stream);
+  if (current != context->device) cudaSetDevice(current);
+  if (status != cudaSuccess) return cuda_failure("MXFP4 synchronize failed", status);
+  volatile uint32_t* word = context->pointer_error();
+  if (*word == 0) return LLMOPT_CUDA_OK;
+  if (clear) *word = 0;
+  return set_error(LLMOPT_CUDA_FAILURE, "a bounded wait inside an MXFP4 product on raw pointers ran out (results are invalid)");
 }
 
 namespace llmopt {

@@ -121,6 +121,7 @@ SIGNATURES = {
     "llmopt_cuda_mxfp4_dequantize": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _P]),
     "llmopt_cuda_mxfp4_linear": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P]),
     "llmopt_cuda_mxfp4_expert_rows": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P]),
+    "llmopt_cuda_mxfp4_synchronize": (_I, [_P, _P, _I]),
     "llmopt_cuda_attention_q8_paged_static": (_I, [_P, _P, _P, _P, _P, _P, _P, _SZ, ctypes.c_uint32, _P]),
     "llmopt_cuda_time_dispatch": (_I, [_P, _REC, _I, _I, _I, ctypes.POINTER(ctypes.c_float)]),
     "llmopt_cuda_time_dispatches": (_I, [_P, _REC, _SZ, _I, _I, ctypes.POINTER(ctypes.c_float)]),
@@ -439,6 +440,10 @@ class Runtime:
         _check(load_library().llmopt_cuda_mxfp4_expert_rows(
             self._context, self._ELEMENTS[element], x_codes_ptr, x_scales_ptr, w_codes_ptr, w_scales_ptr, plan_ptr,
             score_of_slot_ptr or None, out_ptr, slots, n, k, experts, int(paired), stream or None))
+
+    def mxfp4_synchronize(self, stream: int = 0, clear: bool = False) -> None:
+        """Waits for ``stream``; fails if a wait inside a kernel of the pointer forms has run out since the last ``clear``."""
+        _check(load_library().llmopt_cuda_mxfp4_synchronize(self._context, stream or None, int(clear)))
 
     def __del__(self):
         lib = _lib

@@ -66,6 +66,76 @@ def test_sums_of_expert_rows_are_fp32_whatever_the_type(runtime, element):
     check(y.cpu().double().numpy(), want, limit)
 
 
+def whole_numbers(rng, m, n, k):
+    """Operands of a product whose sums fp32 holds, on the GPU, and the product."""
+    pick = np.array([0, 2, 4, 5, 10, 12, 13], np.uint8)
+    x, w = rng.choice(pick, (m, k)), rng.choice(pick, (n, k))
+    ones = [np.full((rows, k // 32), 127, np.uint8) for rows in (m, n)]
+    want = mx.values(x, ones[0]).astype(np.float32) @ mx.values(w, ones[1]).astype(np.float32).T
+    return [on_gpu(a) for a in (mx.pack(x), mx.words(ones[0]), mx.pack(w), mx.words(ones[1]))], want
+
+
+# streams of one CTA per tile, longer and shorter than their ring, and of clusters; pairs of CTAs with one tile each and with several
+SHAPES = [(3, 4096, 4096), (64, 2048, 8192), (20, 40000, 1024), (5, 300, 96), (300, 2304, 2048), (129, 18944, 1536), (100, 256, 96)]
+
+
+@pytest.mark.parametrize("limit", [0, 1, 2])
+def test_products_that_give_up_say_so_to_whoever_waits_for_pointers(runtime, monkeypatch, limit):
+    """A context whose kernels look at a barrier ``limit`` times: products that have to wait longer are reported, by the wait for pointers
+    alone, to everybody until it is cleared; the others are right, and so is everything that runs after them."""
+    import torch
+
+    from llmopt_b200.cuda_native import NativeError, Runtime
+
+    monkeypatch.setenv("LLMOPT_CUDA_MXFP4_WAIT_LIMIT", str(limit))
+    hasty = Runtime()
+    rng = np.random.default_rng(limit)
+    stream = torch.cuda.Stream()
+    for m, n, k in SHAPES:
+        operands, want = whole_numbers(rng, m, n, k)
+        results = [torch.zeros(m, n, device="cuda") for _ in range(4)]
+        torch.cuda.synchronize()
+        call = lambda which, y, s: which.mxfp4_linear_pointers("f32", *[t.data_ptr() for t in operands], None, y.data_ptr(), m, n, k, s)
+        for y in results[:3]:
+            call(hasty, y, stream.cuda_stream)
+        stream.synchronize()
+        hasty.synchronize()  # has another stream and another word
+        try:
+            hasty.mxfp4_synchronize(stream.cuda_stream)
+            gave_up = False
+        except NativeError as error:
+            assert "ran out" in str(error)
+            gave_up = True
+        if limit == 0:
+            assert gave_up
+        if gave_up:
+            for clear in (False, True):
+                with pytest.raises(NativeError, match="ran out"):
+                    hasty.mxfp4_synchronize(0, clear=clear)
+        else:
+            assert all(np.array_equal(y.cpu().numpy(), want) for y in results[:3])
+        hasty.mxfp4_synchronize(stream.cuda_stream)
+        call(runtime, results[3], stream.cuda_stream)
+        runtime.mxfp4_synchronize(stream.cuda_stream)
+        assert np.array_equal(results[3].cpu().numpy(), want)
+
+
+def test_a_batch_that_gives_up_says_so_to_the_context(runtime, monkeypatch):
+    from llmopt_b200 import dispatch
+    from llmopt_b200.cuda_native import NativeError, Runtime
+
+    monkeypatch.setenv("LLMOPT_CUDA_MXFP4_WAIT_LIMIT", "0")
+    hasty = Runtime()
+    rng = np.random.default_rng(3)
+    for m in (3, 300):
+        x, w = ((rng.integers(0, 16, (rows, 1024)).astype(np.uint8), np.full((rows, 32), 127, np.uint8)) for rows in (m, 256))
+        xt, wt, y = upload(hasty, x), upload(hasty, w), blank(hasty, (m, 256), "float32")
+        with pytest.raises(NativeError, match="bounded wait"):
+            dispatch.dispatch_mxfp4_linear(context(hasty), input=xt[0], input_scales=xt[1], weight=wt[0], weight_scales=wt[1], output=y)
+        hasty.synchronize()
+        hasty.mxfp4_synchronize()
+
+
 def cudart():
     """The CUDA runtime that torch has loaded."""
     import ctypes

@@ -1,5 +1,7 @@
 """Calls of the MXFP4 operators at the ends of what they take, as far as they need no GPU."""
 
+import threading
+
 import pytest
 
 
@@ -27,3 +29,14 @@ def test_a_product_of_any_size_is_recorded(m, n, k):
     dispatch.dispatch_mxfp4_linear(dispatch.Context(runtime), input=tensor((m, k // 2), "uint8"), input_scales=tensor((words, m), "uint32"),
                                    weight=tensor((n, k // 2), "uint8"), weight_scales=tensor((words, n), "uint32"), output=tensor((m, n), "float16"))
     assert runtime.records == ["llmopt_mxfp4_linear_f16"]
+
+
+def test_the_wait_for_pointers_needs_a_context():
+    from llmopt_b200 import cuda_native
+
+    lib, got = cuda_native.load_library(), []
+    call = lambda: got.extend([lib.llmopt_cuda_mxfp4_synchronize(None, None, 0), lib.llmopt_cuda_last_error()])
+    thread = threading.Thread(target=call)  # messages are kept per thread
+    thread.start()
+    thread.join()
+    assert got == [1, b"CUDA context has been finalized"]
