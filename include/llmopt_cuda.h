@@ -265,7 +265,8 @@ int llmopt_cuda_measure_hardware(int device, int warmup, int repeats, int64_t by
 /* native/metal_runtime.cpp:58-136 `w4a16_linear(input, packed_weight, scale, bias)`
  * on raw device pointers: input [m,k] f16, packed [n,k/2] u8, scale [n,k/64] f16,
  * bias [n] f16 or NULL, output [m,n] f16; runs on `stream` (a cudaStream_t, may
- * be NULL for the default stream) and does not synchronise. */
+ * be NULL for the default stream, whose work so far it comes after, as after what
+ * the context has been given) and does not synchronise. */
 int llmopt_cuda_w4a16_linear(llmopt_cuda_context* context, const void* input, const void* packed_weight,
                              const void* scale, const void* bias, void* output, int64_t m, int64_t n, int64_t k,
                              void* stream);

@@ -105,6 +105,7 @@ struct Context {
   int device = 0;
   int sm_count = 0;
   cudaStream_t stream = nullptr;
+  cudaEvent_t joined = nullptr;  // where the default stream and this one wait for one another
   std::string name;
   // scratch blocks are only ever added; captured graphs keep pointing at old ones
   std::vector<void*> scratch_blocks;
@@ -181,6 +182,7 @@ static void release(Context* context) {
   if (context->flush_buffer) cudaFree(context->flush_buffer);
   if (context->argmax_result) cudaFree(context->argmax_result);
   if (context->device_error) cudaFreeHost(context->device_error);
+  if (context->joined) cudaEventDestroy(context->joined);
   if (context->stream) cudaStreamDestroy(context->stream);
   delete static_cast<llmopt_cuda_context*>(context);
 }
@@ -809,7 +811,8 @@ int llmopt_cuda_create_context(int device, llmopt_cuda_context** out) {
     delete context;
     return cuda_failure("cudaStreamCreate failed", status);
   }
-  status = cudaMalloc((void**)&context->argmax_result, sizeof(int));
+  status = cudaEventCreateWithFlags(&context->joined, cudaEventDisableTiming);
+  if (status == cudaSuccess) status = cudaMalloc((void**)&context->argmax_result, sizeof(int));
   if (status == cudaSuccess) status = cudaHostAlloc((void**)&context->device_error, 2 * sizeof(uint32_t), cudaHostAllocMapped);
   if (status == cudaSuccess) context->device_error[0] = context->device_error[1] = 0;
   if (status != cudaSuccess) {
@@ -1615,7 +1618,23 @@ int llmopt_cuda_w4a16_linear(llmopt_cuda_context* context, const void* input, co
   args.error = &message;
   if (launch_w4a16_linear == nullptr)
     return set_error(LLMOPT_CUDA_FAILURE, "this library was linked without the W4A16 kernels");
-  if (launch_w4a16_linear(args) != 0) return set_error(LLMOPT_CUDA_FAILURE, message);
+  // The default stream: the call runs on the context's, whose buffers and scratch it may use, after what the default stream has been given
+  // and ahead of what it is given next.
+  int current = -1;
+  if (!stream) {
+    CUDA_TRY(cudaGetDevice(&current), "cudaGetDevice failed");
+    if (current != context->device) CUDA_TRY(cudaSetDevice(context->device), "cudaSetDevice failed");
+  }
+  auto join = [&](cudaStream_t first, cudaStream_t then) {
+    const cudaError_t status = cudaEventRecord(context->joined, first);
+    return status != cudaSuccess ? status : cudaStreamWaitEvent(then, context->joined, 0);
+  };
+  cudaError_t status = stream ? cudaSuccess : join(cudaStreamLegacy, context->stream);
+  const int refused = status == cudaSuccess ? launch_w4a16_linear(args) : 0;
+  if (!stream && status == cudaSuccess) status = join(context->stream, cudaStreamLegacy);
+  if (!stream && current != context->device) cudaSetDevice(current);
+  if (status != cudaSuccess) return cuda_failure("w4a16_linear on the default stream", status);
+  if (refused != 0) return set_error(LLMOPT_CUDA_FAILURE, message);
   return LLMOPT_CUDA_OK;
 }
 
