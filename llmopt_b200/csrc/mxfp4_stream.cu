@@ -30,8 +30,8 @@ struct Shape {
   static constexpr uint32_t kStageBytes = kInputScalesAt + kStageWords * kAtom;
   static constexpr uint32_t kStages = 4;  // at most
   static constexpr uint32_t kScaleColumns = kStageWords * 8;
-  static constexpr uint32_t kUsedColumns = NT + 2 * kScaleColumns;
-  static constexpr uint32_t kTmemColumns = kUsedColumns <= 128 ? 128 : 256;
+  static constexpr uint32_t kTmemColumns = 128;
+  static_assert(NT + 2 * kScaleColumns <= kTmemColumns, "tensor memory");
   static constexpr uint32_t kHolder = (3 * kStages + 2) * 8;  // behind the ring: barriers, tensor memory's address, abort flag
   static constexpr uint32_t kBehind = kHolder + 8;
   static constexpr uint32_t kPiece = NT == 16 ? 16 : 32;
