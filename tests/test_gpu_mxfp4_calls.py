@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import mxfp4_oracle as mx
-from test_gpu_mxfp4 import HALF_STEP, allowed, blank, check, context, device, expert_case, from_bits, read, upload
+from test_gpu_mxfp4 import HALF_STEP, allowed, blank, check, context, device, expert_case, from_bits, read, special_rows, upload
 
 pytestmark = pytest.mark.gpu
 
@@ -40,6 +40,36 @@ def test_pairs_with_gates_far_from_zero(runtime, dtype, slots, k):
     check(got[~beyond], want[~beyond], limit[~beyond])
 
 
+@pytest.mark.parametrize("counts,n,k", [([3, 5, 0, 9], 130, 416), ([3, 5, 9], 200, 4096), ([100, 200, 40], 96, 288), ([130, 300, 20], 300, 2080)])
+def test_blocks_of_nan_among_sorted_rows_reach_their_row_or_column_alone(runtime, counts, n, k):
+    """Rows of another expert, and another expert's columns, lie in the same boxes."""
+    from llmopt_b200 import dispatch
+
+    rng = np.random.default_rng(len(counts) + k)
+    expert_of_slot, x, w, score = expert_case(rng, counts, n, k)
+    slots, ends = len(expert_of_slot), np.cumsum(counts)
+    x = x[0], (x[1] - 4).astype(np.uint8)
+    x[1][ends[0] - 1, -1] = x[1][ends[1], 0] = 255  # the last row of one expert, the first of the one after the next
+    w[1][n, 1] = w[1][2 * n - 1, -1] = 255          # the second expert's first and last column
+    xv, wv = mx.values(*x), mx.values(*w).reshape(len(counts), n, k)
+    bad = np.isnan(xv).any(1)[:, None] | np.isnan(wv).any(2)[expert_of_slot]
+    xn, wn = np.nan_to_num(xv), np.nan_to_num(wv)
+    want, limit = np.zeros((slots, n)), np.zeros((slots, n))
+    for e in range(len(counts)):
+        mine = expert_of_slot == e
+        want[mine] = xn[mine] @ wn[e].T
+        limit[mine] = allowed(xn[mine], wn[e], want[mine], "float32")
+    xt, wt = upload(runtime, x), upload(runtime, w)
+    plan = device(runtime, mx.plan_of(expert_of_slot, len(counts)))
+    operands = dict(input=xt[0], input_scales=xt[1], weight=wt[0], weight_scales=wt[1], experts=len(counts), plan=plan.buffer)
+    y = blank(runtime, (slots, n), "float32", 256)
+    dispatch.dispatch_mxfp4_expert_rows(context(runtime), **operands, output=y)
+    check(read(y, 256).astype(np.float64), np.where(bad, np.nan, want), limit)
+    y = blank(runtime, (slots, n // 2), "bfloat16", 256)
+    dispatch.dispatch_mxfp4_expert_rows(context(runtime), **operands, output=y, score_of_slot=device(runtime, score))
+    assert np.array_equal(np.isnan(from_bits(read(y, 256), "bfloat16")), bad[:, 0::2] | bad[:, 1::2])
+
+
 # ---- raw pointers -----------------------------------------------------------------------------------------
 
 def on_gpu(array):
@@ -64,6 +94,59 @@ def test_sums_of_expert_rows_are_fp32_whatever_the_type(runtime, element):
     want = np.einsum("sk,snk->sn", xv, wv[expert_of_slot])
     limit = np.stack([allowed(xv[i:i + 1], wv[e], want[i:i + 1], "float32")[0] for i, e in enumerate(expert_of_slot)])
     check(y.cpu().double().numpy(), want, limit)
+
+
+def guarded(shape, dtype, behind=64):
+    """A tensor on the GPU with bytes of canaries in it and behind it, and what says that those behind are as they were."""
+    import torch
+
+    count = int(np.prod(shape)) * torch.empty(0, dtype=dtype).element_size()
+    whole = torch.full((count + behind,), 0xA5, dtype=torch.uint8, device="cuda")
+    return whole[:count].view(dtype).reshape(shape), lambda: bool((whole[count:] == 0xA5).all())
+
+
+@pytest.mark.parametrize("element,dtype", [("f16", "float16"), ("bf16", "bfloat16"), ("f32", "float32")])
+def test_gathered_rows_of_pointers(runtime, element, dtype):
+    """Fewer and more slots than rows, rows further apart than they are long, an index beyond them."""
+    import torch
+
+    rng = np.random.default_rng(51)
+    stream = torch.cuda.current_stream().cuda_stream
+    for slots, source, k, stride in ((9, 40, 160, 161), (70, 5, 576, 640), (1, 1, 32, 32)):
+        bits = special_rows(rng, source, k, dtype)
+        index = rng.integers(0, source, slots).astype(np.uint32)
+        index[-1] = source - 1
+        beyond = index.copy()
+        beyond[-1] = source + 7
+        wide = np.concatenate([bits, np.full((source, stride - k), 0x7F, bits.dtype)], axis=1)
+        x, rows = on_gpu(wide.view({2: np.int16, 4: np.int32}[wide.itemsize])), on_gpu(beyond)
+        (codes, codes_kept), (scales, scales_kept) = guarded((slots, k // 2), torch.uint8), guarded(((k + 127) // 128, slots), torch.int32)
+        runtime.mxfp4_quantize_pointers(element, x.data_ptr(), rows.data_ptr(), codes.data_ptr(), scales.data_ptr(), slots, source, k, stride, stream)
+        nibbles, exponents = mx.quantize(from_bits(bits, dtype)[index])
+        assert np.array_equal(mx.exponents(scales.cpu().numpy().view(np.uint32), k), exponents) and scales_kept()
+        assert np.array_equal(mx.unpack(codes.cpu().numpy()), nibbles) and codes_kept()
+
+
+@pytest.mark.parametrize("element,dtype", [("f16", "float16"), ("bf16", "bfloat16")])
+def test_pairs_of_pointers(runtime, element, dtype):
+    """The same bits as a dispatch of the kernel, whose results are compared with the definition, and none behind them."""
+    import torch
+
+    from llmopt_b200 import dispatch
+
+    rng = np.random.default_rng(52)
+    stream = torch.cuda.current_stream().cuda_stream
+    for counts, n, k in (([3, 0, 9], 64, 160), ([150, 1, 0, 60], 202, 2048)):
+        expert_of_slot, x, w, score = expert_case(rng, counts, n, k)
+        x = x[0], (x[1] - 4).astype(np.uint8)
+        slots, plan = len(expert_of_slot), mx.plan_of(expert_of_slot, len(counts))
+        xt, wt, want = upload(runtime, x), upload(runtime, w), blank(runtime, (slots, n // 2), dtype)
+        dispatch.dispatch_mxfp4_expert_rows(context(runtime), input=xt[0], input_scales=xt[1], weight=wt[0], weight_scales=wt[1], experts=len(counts),
+                                            plan=device(runtime, plan).buffer, output=want, score_of_slot=device(runtime, score))
+        held = [on_gpu(a) for a in (mx.pack(x[0]), mx.words(x[1]), mx.pack(w[0]), mx.words(w[1]), plan, score)]
+        y, kept = guarded((slots, n // 2), torch.int16)
+        runtime.mxfp4_expert_rows_pointers(element, *[t.data_ptr() for t in held], y.data_ptr(), slots, n, k, len(counts), True, stream)
+        assert np.array_equal(y.cpu().numpy().view(np.uint16), read(want)) and kept()
 
 
 def whole_numbers(rng, m, n, k):
