@@ -3,7 +3,9 @@ kernel of their steps: the recurrent design beside the W4A16 decoder of the same
 and the like kernels of that path, the windowed design with routed experts beside the recurrent one.  Used by
 ``bench.py --mixers``; random weights.
 
-  python -m llmopt_b200.mixer_bench [--design bizodra|dalorax] [--size 2048|4096|all] [--tokens 2048] [--context 2048]"""
+  python -m llmopt_b200.mixer_bench [--design bizodra|dalorax] [--size 2048|4096|all] [--tokens 2048] [--context 2048] [--experts mxfp4]
+
+With ``--experts mxfp4`` the windowed design also with its routed experts in four bits, and how far its logits are from the others."""
 
 from __future__ import annotations
 
@@ -67,7 +69,7 @@ def like_config(config: MixerConfig) -> ModelConfig:
 
 def experts_in_use(item) -> int:
     """Experts that some row of an expert kernel's step chose, from its device-side route or plan."""
-    words = item.buffers[2].to_numpy(np.uint32)
+    words = item.buffers[4 if "mxfp4" in item.name else 2].to_numpy(np.uint32)
     if "expert_step" in item.name:
         return int(words[0])
     return len(set(words[4:4 + 4 * int(words[0])].reshape(-1, 4)[:, 0].tolist()))
@@ -98,6 +100,13 @@ def work_of(item, past: int, itemsize: int):
         pairs, n, k, experts, paired = u
         return (f"expert_rows n{n} k{k}", (experts_in_use(item) * n * k + pairs * k) * e + pairs * n * (e // 2 if paired else 4),
                 2 * pairs * n * k)
+    if stem == "mxfp4_expert_rows":
+        pairs, n, k, experts, paired = u
+        return (f"{stem} n{n} k{k}", (experts_in_use(item) * n + pairs) * (k // 2 + k // 32) + pairs * n * (1 if paired else 4),
+                2 * pairs * n * k)
+    if stem in ("mxfp4_quantize", "mxfp4_quantize_rows"):
+        rows, k = u[:2]
+        return f"{stem} k{k}", (u[3] if "rows" in stem else rows) * k * e + rows * (k // 2 + k // 32), 0
     if stem in ("route_step", "route_rows", "route_plan"):
         rows, experts, top = u
         return stem, rows * (experts * 4 if stem != "route_plan" else top * 8) + rows * top * (8 if stem != "route_plan" else 12), 0
@@ -157,7 +166,7 @@ def time_items(runtime, items, past: int, itemsize: int, peaks: dict) -> dict:
         groups.setdefault(work_of(item, past, itemsize)[0], []).append(item)
     table = {}
     for label, group in groups.items():
-        if label.startswith(("route", "expert")):
+        if label.startswith(("route", "expert", "mxfp4_expert")):
             runtime.time_dispatches(items, warmup=0, iterations=1)  # routes of a whole step, not of what was timed before
         launches = len(group)
         ms = runtime.time_dispatches(group * max(1, min(16, 64 // launches)), warmup=2, iterations=5)
@@ -165,7 +174,7 @@ def time_items(runtime, items, past: int, itemsize: int, peaks: dict) -> dict:
         floor = max(nbytes / peaks["hbm_gbs"] / 1e6, flops / peaks["bf16_tflops"] / 1e9)
         table[label] = {"launches": launches, "us": round(ms * 1e3, 2), "floor_us": round(floor * 1e3, 2),
                         "frac": round(floor / ms, 3) if ms else None, "share_us": round(ms * 1e3 * launches, 1)}
-        if label.startswith("expert") and "combine" not in label:
+        if label.startswith(("expert", "mxfp4_expert")) and "combine" not in label:
             table[label]["experts_in_use"] = experts_in_use(group[0])
     return table
 
@@ -200,14 +209,30 @@ def prefill_rate(engine, tokens: int) -> dict:
     return {"tokens": tokens, "ms": round(seconds * 1e3, 3), "tokens_per_s": round(tokens / seconds, 1)}
 
 
-def measure_mixers(runtime, peaks: dict, config: MixerConfig, tokens: int, context: int, batches=(1, 8, 32)) -> dict:
+def logits_distance(runtime, config: MixerConfig, weights, tokens: int, experts: str) -> dict:
+    """Logits at every place of a prompt with experts in a format of their own, beside those of the model as it is: the differences' share of
+    the spread (root of the mean squares)."""
+    from .mixer_engine import MixerEngine
+
+    prompt = np.random.default_rng(1).integers(0, config.vocabulary, size=tokens).tolist()
+    seen = []
+    for options in ({}, {"experts": experts}):
+        engine = MixerEngine(runtime, config, weights, capacity=tokens + 16, prompt_rows=tokens, **options)
+        seen.append(engine.run([(engine.open(), prompt, range(tokens))])[0])
+    spread = seen[0] - seen[0].mean(axis=1, keepdims=True)
+    return {"tokens": tokens, "off": round(float(np.sqrt(np.mean((seen[1] - seen[0]) ** 2) / np.mean(spread ** 2))), 4)}
+
+
+def measure_mixers(runtime, peaks: dict, config: MixerConfig, tokens: int, context: int, batches=(1, 8, 32), experts=None) -> dict:
     from .mixer_engine import MixerEngine
 
     weights = random_mixer_weights(config, seed=0, fast=True)
     result = {"model": config.name, "width": config.width, "layers": len(config.layers), "decode": [], "kernels": {}}
+    if experts:
+        result.update(experts=experts, logits=logits_distance(runtime, config, weights, min(tokens, 512), experts))
     for batch in batches:
         engine = MixerEngine(runtime, config, weights, batch=batch, capacity=context + 64 + (tokens if batch == 1 else 0),
-                             prompt_rows=tokens if batch == 1 else batch)
+                             prompt_rows=tokens if batch == 1 else batch, experts=experts)
         result["decode"].append(decode_rate(engine, batch, context))
         plan = engine._decode_plan(batch)[0]
         engine.rewind(context)
@@ -304,12 +329,14 @@ def like_kernels(runtime, peaks: dict, config: MixerConfig, tokens: int, context
 
 
 def measure(runtime, peaks: dict, widths=(2048, 4096), tokens: int = 2048, context: int = 2048, like: bool = True,
-            design: str = "bizodra") -> list:
+            design: str = "bizodra", experts=None) -> list:
     results = []
     for width in widths:
         config = sized_config(width)
         if design == "dalorax":
             entry = {"windows": measure_mixers(runtime, peaks, windowed_config(width), tokens, context)}
+            if experts:
+                entry[f"windows, experts in {experts}"] = measure_mixers(runtime, peaks, windowed_config(width), tokens, context, experts=experts)
             if like:
                 entry["mixers"] = measure_mixers(runtime, peaks, config, tokens, context)
         else:
@@ -328,10 +355,13 @@ def main() -> None:
     parser.add_argument("--tokens", type=int, default=2048)
     parser.add_argument("--context", type=int, default=2048)
     parser.add_argument("--no-like", action="store_true", help="only the design itself")
+    parser.add_argument("--experts", default=None, choices=["mxfp4"], help="format of routed experts' weights (dalorax)")
     args = parser.parse_args()
+    if args.experts and args.design != "dalorax":
+        parser.error("only the dalorax design has routed experts")
     peaks = {"hbm_gbs": 6531.6, "bf16_tflops": 1657.8}
     widths = (2048, 4096) if args.size == "all" else (int(args.size),)
-    for entry in measure(Runtime(), peaks, widths, args.tokens, args.context, not args.no_like, args.design):
+    for entry in measure(Runtime(), peaks, widths, args.tokens, args.context, not args.no_like, args.design, args.experts):
         print(json.dumps(entry, indent=1))
 
 
