@@ -70,6 +70,52 @@ def test_blocks_of_nan_among_sorted_rows_reach_their_row_or_column_alone(runtime
     assert np.array_equal(np.isnan(from_bits(read(y, 256), "bfloat16")), bad[:, 0::2] | bad[:, 1::2])
 
 
+@pytest.mark.parametrize("m", [2, 70])
+def test_the_longest_rows(runtime, m):
+    """k of 2^23, the most that is taken: single elements here and there, whose products fp32 holds."""
+    import torch
+
+    k, n = 1 << 23, 5
+    rng = np.random.default_rng(m)
+    places = np.unique(np.concatenate([[0, 1, 31, 32, 511, 512, k // 2 - 1, k // 2, k - 1], rng.integers(0, k, 40)]))
+    pick = np.array([2, 4, 5, 10, 12], np.uint8)  # 1, 2, 3, -1, -2
+    value = np.array([0.0, 0.0, 1.0, 0.0, 2.0, 3.0, 0.0, 0.0, 0.0, 0.0, -1.0, 0.0, -2.0])
+
+    def rows(count):
+        nibbles = rng.choice(pick, (count, len(places)))
+        codes = torch.zeros(count, k // 2, dtype=torch.uint8, device="cuda")
+        for column, place in enumerate(places):
+            codes[:, place // 2] |= on_gpu(nibbles[:, column] << (4 * (place % 2)))
+        return value[nibbles], codes, torch.full((k // 128, count), 0x7F7F7F7F, dtype=torch.int32, device="cuda")
+
+    (xv, x, xs), (wv, w, ws) = rows(m), rows(n)
+    y = torch.zeros(m, n, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    runtime.mxfp4_linear_pointers("f32", x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), None, y.data_ptr(), m, n, k, stream)
+    assert np.array_equal(y.cpu().numpy(), xv @ wv.T)
+    with pytest.raises(ValueError, match="too large"):
+        runtime.mxfp4_linear_pointers("f32", x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), None, y.data_ptr(), 1, 1, k + 32, stream)
+
+
+def test_as_many_experts_as_there_can_be(runtime):
+    """8192 of them, most with a row or two, some with none."""
+    from llmopt_b200 import dispatch
+
+    rng = np.random.default_rng(61)
+    experts, n, k = 8192, 6, 64
+    pick = np.array([0, 2, 4, 5, 10, 12, 13], np.uint8)
+    counts = rng.integers(0, 3, experts)
+    counts[-1] = 1
+    expert_of_slot = np.repeat(np.arange(experts), counts)
+    slots = len(expert_of_slot)
+    x, w = ((rng.choice(pick, (rows, k)), np.full((rows, 2), 127, np.uint8)) for rows in (slots, experts * n))
+    want = np.einsum("sk,snk->sn", mx.values(*x), mx.values(*w).reshape(experts, n, k)[expert_of_slot])
+    xt, wt, y = upload(runtime, x), upload(runtime, w), blank(runtime, (slots, n), "float32", 256)
+    dispatch.dispatch_mxfp4_expert_rows(context(runtime), input=xt[0], input_scales=xt[1], weight=wt[0], weight_scales=wt[1], experts=experts,
+                                        plan=device(runtime, mx.plan_of(expert_of_slot, experts)).buffer, output=y)
+    assert np.array_equal(read(y, 256), want)
+
+
 # ---- raw pointers -----------------------------------------------------------------------------------------
 
 def on_gpu(array):
