@@ -13,8 +13,9 @@ namespace llmopt {
 namespace {
 using namespace mxfp4;
 
-// Both are bound by HBM, few rows by the launch: values of 14336 x 4096 fp32 into codes 45 us, 5.7 TB/s, and back 45 to 49, 5.1 to 5.7;
-// 4096 rows gathered from 2048 x 4096 bf16 10.0; 1 x 4096 2.6.  All of a CTA's values are asked for before the first is looked at.
+// 32-bit values are bound by HBM, 16-bit ones by their instructions (61 % of the issue slots), few rows by the launch: 14336 x 4096 fp32 into
+// codes 45 us, 5.7 TB/s, and back 45 to 49, 5.1 to 5.7; 4096 rows gathered from 2048 x 4096 bf16 10.0, and back 9.5, one behind the other 16.5;
+// 1 x 4096 2.6, and back beside it.  All of a CTA's values are asked for before the first is looked at.
 // A CTA takes 32 rows x 256 columns, a warp four of the rows, 16 bytes of values per lane and access: 256 columns of 16 bits at a
 // time, 128 of 32.  The exponents of the 32 rows leave together, 128 bytes of a word's row.
 constexpr uint32_t kTileRows = 32, kTileColumns = 256, kWarps = 8, kRowsPerWarp = kTileRows / kWarps;

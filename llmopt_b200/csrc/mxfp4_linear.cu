@@ -27,7 +27,10 @@ int run_product(const KernelArgs& args, const Problem& p, uint32_t plan_tiles) {
   // through 4096 x 7168 25.7, 28.2.  Tiles that would be more than 13 CTAs for every two SMs go to the kernel whose CTAs stay for the next
   // (stream, tiles: 448 tiles, 32 rows through 4096 x 57344 26.7, 28.7; 896, 64 sorted rows through 4096 x 7168 37.2, 36.7; 1002, 4096 x 128256
   // 32 rows 53.6, 51.8, 64 rows 58.3, 54.4; 1024, 64 sorted rows of 64 experts 15.6, 14.8; 7168, 64 of 128 experts 110, 80), unless all read the
-  // same rows and those are few (1 row through 4096 x 128256 48.8, 50.0, 16 rows 51.6, 51.1).
+  // same rows and those are few (1 row through 4096 x 128256 48.8, 50.0, 16 rows 51.6, 51.1).  Between, by how the tiles fill the last round
+  // of the stream's two CTAs per SM (32 and 64 rows, in another series): 512 tiles 28.0, 29.1 and 29.0, 29.6; 640 36.1, 35.4 and 37.8, 36.1; 768
+  // 40.1, 41.1 and 41.9, 42.3; 896 47.2, 46.7 and 49.5, 48.2.  With small k the line would lie lower: k 1024, 64 rows, 448 10.9, 10.4, 896
+  // 17.9, 15.8.
   const uint64_t tiles = (uint64_t)(p.plan.tiles ? plan_tiles : 1u) * ((p.n + kColumns - 1u) / kColumns);
   const bool few = tiles * 2u <= (uint64_t)context_sm_count(args.ctx) * 13u || (!p.plan.tiles && p.m <= 16u);
   return p.m <= 64u && few ? run_stream<S>(args, p, plan_tiles) : run_tiles<S>(args, p, plan_tiles);

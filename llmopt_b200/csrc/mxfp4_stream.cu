@@ -5,12 +5,13 @@
 // registers and laid down in the order that tcgen05.cp spreads over tensor memory; one lane of warp 1 issues copies and products; then
 // warps 2 to 5 read the sums out.  CTAs of a cluster hand each row's sums to the one that joins them, in the order of k.
 //
-// The copies start before the block's other warps: the barriers are warp 0's own until it says that they are there.  One pass: 57344 x
-// 14336 1 row 71 us (6.2 TB/s), 64 rows 77; 128256 x 4096 1 row 48.4 (5.8); 14336 x 4096 1 row 8.5, where the launch, the first copies'
-// latency and the way out are half of it; 4096 x 4096 5.6.  Stages of 256 had the same bytes in flight and twice the handovers, 485 cycles
-// each, more than the copies of a stage take.  Asking for the weights while the previous kernel ends made both slower.
+// The copies start before the block's other warps: the barriers are warp 0's own until it says that they are there.  Weights cold, calls of a
+// kind behind one another (k x columns, as everywhere here): 14336 x 57344 1 row 68 to 75 us (6.4 to 5.8 TB/s, by GPU); 4096 x 128256 46 to 50;
+// 4096 x 14336 7.8, 64 rows 8.8, where the launch, the first copies' latency and the way out are half of it; 14336 x 4096 8.3, 4096 x 4096 4.7.
+// Stages of 256 had the same bytes in flight and twice the handovers, 485 cycles each, more than the copies of a stage take.  Asking for the
+// weights while the previous kernel ends made both slower.
 //
-// Every wait on an mbarrier is bounded; a wait that runs out raises the context's device error word, and the CTA lets its copies and
+// Every wait on an mbarrier is bounded; a wait that runs out raises the launch's error word, and the CTA lets its copies and
 // products end, frees its tensor memory and returns.
 #include "mxfp4_tc.cuh"
 
@@ -315,11 +316,11 @@ int run(const KernelArgs& args, const Problem& p, uint32_t row_tiles) {
   const size_t tiles = (size_t)work.row_tiles * work.column_tiles;
   LLMOPT_REQUIRE(tiles < (1u << 28), "too many tiles");
   // CTAs that share a tile's k while tiles leave SMs without work; powers of two, which leave the fewest SMs of a GPC over.  us with 1, 2, 4, 8
-  // of them: 4096 x 4096 5.9, 5.2, 4.5, 6.2; k 14336 x 4096 14.6, 10.2, 8.6, 17; 4096 x 14336 (112 tiles) 7.6, 11.8.
+  // of them: 4096 x 4096 6.1, 5.3, 4.7, 6.0; 14336 x 4096 15.0, 9.9, 8.3, 10.0; 4096 x 14336 (112 tiles) 7.9, 9.4.
   while (work.splits < kMostSplits && tiles * work.splits * 2u <= sms && p.k / kDepth >= work.splits * 2u) work.splits *= 2u;
   const uint32_t mine = (k_stages + work.splits - 1u) / work.splits;
-  // a CTA per SM: a deep ring; more: two of them per SM, which start and end beside one another (4 and 2 stages: 4096 x 14336 7.6, 9.0 us;
-  // 4096 x 128256 60.6, 50.7)
+  // a CTA per SM: a deep ring; more: two of them per SM, which start and end beside one another (4 and 2 stages: 4096 x 14336 7.8, 9.1 us,
+  // 14336 x 4096 8.3, 9.5; 4096 x 128256 56.3, 49.7)
   const uint32_t most = tiles * work.splits <= sms ? Z::kStages : 2u;
   work.stages = mine < most ? mine : most;
   const uint32_t rows = p.m < NT ? p.m : NT;
