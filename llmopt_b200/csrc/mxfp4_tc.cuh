@@ -88,17 +88,18 @@ template <> struct Element<kStorePairBf16> { typedef bf16 Type; };
 __device__ __forceinline__ uint32_t packed(__half a, __half b) { return (uint32_t)__half_as_ushort(a) | (uint32_t)__half_as_ushort(b) << 16; }
 __device__ __forceinline__ uint32_t packed(bf16 a, bf16 b) { return (uint32_t)__bfloat16_as_ushort(a) | (uint32_t)__bfloat16_as_ushort(b) << 16; }
 
-// silu(gate) up = gate up t^3 / (1 + t^3), t = e^(gate / 3), whose exponential and quotient are off by a few steps of fp32: of a result in
-// sixteen bits that is nothing, and with the exact quotient the pairs of a tile took longer than its products (9.0 against 5.2 us).  Far
-// below zero silu leaves fp32's normal numbers, where `up` may bring it back, so every t is a factor of its own: t stays normal down to a
-// gate of -262, where nothing that fp32 holds is left of the product.  From 18 on the quotient is 1 to less than half a step; t grows no
-// further, so that its cube stays finite.  us of 4096 sorted rows through 4096 x 7168: 72.9; with the square of e^(gate / 2), which needs
-// subnormal numbers, 74.6; silu by itself, zero from -87 on, 71.9.
+// silu(gate) up: gate up / (1 + t^3) with t = e^(-|gate| / 3), below zero times t^3.  Its exponential and quotient are off by a few steps of
+// fp32: of a result in sixteen bits that is nothing, and with the exact quotient the pairs of a tile took longer than its products (9.0
+// against 5.2 us).  Far below zero silu leaves fp32's normal numbers, where `up` may bring it back: so every t is a factor of its own, and
+// either side has one ahead of their product, which leaves fp32's range only if the result does.  t stays normal down to a gate of
+// -262, where nothing that fp32 holds is left of the product.  us of 4096 sorted rows through 4096 x 7168: 73.5; with the square of
+// e^(gate / 2), which needs subnormal numbers, 74.9; silu by itself, zero from -87 on, 72.2.
 __device__ __forceinline__ float silu_pair(float gate, float up) {
   float t, inverse;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fminf(gate, 18.0f) * 0.48089834696f));  // log2(e) / 3
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fabsf(gate) * -0.48089834696f));  // log2(e) / 3
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(fmaf(t * t, t, 1.0f)));
-  return gate * (t * inverse) * up * t * t;
+  const float factor = gate < 0.0f ? t : 1.0f;
+  return (gate * inverse * factor) * (up * factor) * factor;
 }
 
 // Sums of COUNT rows from `row` on, of the output column that is this lane's, and its bias: fp32.

@@ -40,6 +40,33 @@ def test_pairs_with_gates_far_from_zero(runtime, dtype, slots, k):
     check(got[~beyond], want[~beyond], limit[~beyond])
 
 
+@pytest.mark.parametrize("slots,k", [(40, 64), (200, 2048)])
+@pytest.mark.parametrize("power,low,high", [(-125, 1.0, 22.6), (119, 1.0, 22.6), (0, 1.0, 22.6), (-134, 17.0, 80.0)])
+def test_pairs_whose_products_lie_at_the_ends_of_bfloat16(runtime, power, low, high, slots, k):
+    """Results between 2^-126 and 2^128 are normal numbers of bfloat16 with 8 bits each, whatever the factors: nothing on the way may leave
+    fp32's range before they do.  Steps as above, and the other column's by which it is off where it is subnormal; results within half a
+    step of the largest number are left out."""
+    from llmopt_b200 import dispatch
+
+    score = np.geomspace(low, high, slots).astype(np.float32)
+    score[::3] *= -1  # gates below zero
+    n = 34
+    x, w = (np.zeros((slots, k), np.uint8), np.full((slots, k // 32), 127, np.uint8)), (np.zeros((n, k), np.uint8), np.full((n, k // 32), 127, np.uint8))
+    x[0][:, 0], x[0][:, -1], w[0][0::2, 0], w[0][1::2, -1] = 2, 2, 2, 2  # 1 for the gate, from the other end 2^power for the other column
+    x[1][:, -1], w[1][:, -1] = 127 + min(power, 0) // 2, 127 + power - min(power, 0) // 2
+    gate, up = score.astype(np.float64), score.astype(np.float64) * 2.0 ** power
+    want = np.repeat((gate / (1 + np.exp(-gate)) * up)[:, None], n // 2, 1)
+    xt, wt = upload(runtime, x), upload(runtime, w)
+    y = blank(runtime, (slots, n // 2), "bfloat16", 256)
+    dispatch.dispatch_mxfp4_expert_rows(context(runtime), input=xt[0], input_scales=xt[1], weight=wt[0], weight_scales=wt[1], experts=1,
+                                        plan=device(runtime, mx.plan_of(np.zeros(slots, int), 1)).buffer, output=y, score_of_slot=device(runtime, score))
+    limit = np.abs(want) * (HALF_STEP["bfloat16"] * (1 + 2.0 ** -10) + (3 * (2 + 0.75 * np.abs(gate) / 3) + 5)[:, None] * 2.0 ** -23)
+    limit = limit + 2.0 ** -150 * np.abs(want / up[:, None])
+    got, normal = from_bits(read(y, 256), "bfloat16"), (np.abs(want) >= 2.0 ** -126) & (np.abs(want) < 2.0 ** 128 * (1 - 2.0 ** -8))
+    assert normal.mean() > 0.6
+    check(got[normal], want[normal], limit[normal])
+
+
 @pytest.mark.parametrize("counts,n,k", [([3, 5, 0, 9], 130, 416), ([3, 5, 9], 200, 4096), ([100, 200, 40], 96, 288), ([130, 300, 20], 300, 2080)])
 def test_blocks_of_nan_among_sorted_rows_reach_their_row_or_column_alone(runtime, counts, n, k):
     """Rows of another expert, and another expert's columns, lie in the same boxes."""
