@@ -11,7 +11,7 @@
 //
 // What bounds it: a stage costs the tensor cores 4 cycles per row of x and 200 to 500 for copies of exponents (12 of them, in the same
 // pipe) and the handover of the ring.  Stages of 512 rather than 256 elements halve the handovers: 4096 x 4096 x 14336 108 -> 99 us, 2048 x
-// 4096 x 4096 24.9 -> 21.3, 512 x 14336 x 4096 25.7 -> 20.9.  (These three are 92, 19.7 and 19.7 now.)  The large
+// 4096 x 4096 24.9 -> 21.3, 512 x 14336 x 4096 25.7 -> 20.9.  (These three are 92 to 96, 19.7 and 19.8 now.)  The large
 // product runs at up to 5.2 PFLOP/s (k 8192: 5.8) and takes 82 to 87 us where all codes are zero: what is left between the two is power,
 // 1000 W, and repeated for a second it takes 110 at 1.6 to 1.7 GHz.  Rows sorted by expert have tiles of 128, which spend up to half a
 // stage outside the products; many are joined to tiles of up to 224: 4096 of 16 experts through 4096 x 7168 85 -> 73 us, 3.3 PFLOP/s and
@@ -73,7 +73,7 @@ __device__ __forceinline__ void pair_store(uint32_t local, uint32_t rank, uint32
 // with fences restricted to shared memory where that changes hands and tcgen05.fence for tensor memory: release and acquire of
 // everything wait for global memory too.  The warps that bring exponents take part in none of it: even a restricted fence waits for the loads that
 // they have under way, so warp 0 tells them when a stage is theirs, and the second CTA's warp 1 tells the first what they have laid down.
-// us, cold, of 777 x 2048 x 7168, 4096 x 4096 x 14336 and 32 x 4096 x 128256 (fp32): 10.5, 93, 48 to 51; with fences in those warps 10.8, 98, 55; with
+// us, cold, of 777 x 2048 x 7168, 4096 x 4096 x 14336 and 32 x 4096 x 128256 (fp32): 10.5, 92 to 96, 48 to 51; with fences in those warps 10.8, 98, 55; with
 // release and acquire of everything 15.4, 156, 87.
 __device__ __forceinline__ void shared_release() { asm volatile("fence.release.sync_restrict::shared::cta.cluster;" ::: "memory"); }
 __device__ __forceinline__ void first_arrive(uint32_t first) {
